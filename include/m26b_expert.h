@@ -345,6 +345,56 @@ int m26b_frame_parse_return(const uint8_t* frame, uint64_t len, int check_crc, u
 int m26b_plan_static(const int32_t* ids, const float* weights, uint32_t rows, int32_t* inverse, int32_t* original_routes,
                      float* grouped_weights, uint32_t* meta_out, void* stream, char* err, size_t errlen);
 
+/* ---- Dense operators around the routed experts -------------------------------------------------------------------
+ * The same checkpoint format outside the expert list: a shared expert, a first dense layer, any projection held in MXFP4.
+ *
+ * A linear handle owns one prepared matrix (y = x W^T), or a gated pair (y = silu(x Wg^T) * (x Wu^T), both projections, the
+ * activation and the product in one kernel).
+ *   new:       w u8 [n][k/2] (E2M1 pairs, low nibble = even k) and s u8 [n][k/32] (UE8M0; byte 255 is stored as 254), device
+ *              memory, dense rows, any alignment; k a multiple of 32, n and k at most 2^20. As m26b_layer_new, the call first
+ *              waits for all work queued on the current device; the sources may be freed when it returns.
+ *   new_gated: the same for gate_proj and up_proj, both [n][k].
+ *   workspace_bytes: device bytes m26b_linear_dev needs for `rows` tokens (0 for 0 rows); grows with rows up to 8,192.
+ *   linear_dev: x [rows][k] with rows x_pitch elements apart, x_dtype 0 = BF16 or 2 = E4M3 with x_scales u8 [rows][k/32]
+ *              (UE8M0, dense) -> y [rows][n] with rows y_pitch elements apart, y_dtype 0 = BF16 (one rounding, nearest even) or
+ *              1 = FP32. A pitch of 0 means dense rows. Only y's n columns of `rows` rows are written. Any number of rows: one
+ *              token to a prefill batch (passes of 8,192); 0 rows is no work. BF16 activations are not quantised: a K32 block
+ *              enters the product as two E4M3 pieces that equal it exactly, save for elements below 2^-14 of the block's
+ *              largest, which carry an error of at most 2^-21 of that largest. Products accumulate in FP32. A row with an
+ *              infinity, a NaN (or, for x_dtype 2, a NaN code or scale byte 255) in it is NaN in all its outputs. A row's
+ *              result does not change with the other rows' values.
+ *              workspace: 128-byte aligned device memory of at least workspace_bytes(rows), one call at a time (calls that
+ *              may overlap, or captured graphs that may run together, each need their own); its content is of no use between
+ *              calls. fault_dev: one u32 that receives code 3 (ORed) if a bounded wait inside the kernel ran out, in which
+ *              case y is undefined. Nothing is allocated, nothing is synchronised, and a call can be captured into a graph;
+ *              the handle must stay alive until the work is done. Enqueued on `stream` (NULL = the default stream). */
+typedef struct m26b_linear m26b_linear;
+int m26b_linear_new(const uint8_t* w, const uint8_t* s, uint32_t n, uint32_t k, m26b_linear** out, char* err, size_t errlen);
+int m26b_linear_new_gated(const uint8_t* gate_w, const uint8_t* gate_s, const uint8_t* up_w, const uint8_t* up_s, uint32_t n, uint32_t k,
+                          m26b_linear** out, char* err, size_t errlen);
+void m26b_linear_free(m26b_linear* l);
+uint64_t m26b_linear_workspace_bytes(const m26b_linear* l, uint32_t rows);
+int m26b_linear_dev(const m26b_linear* l, const void* x, int x_dtype, const uint8_t* x_scales, uint64_t x_pitch, uint32_t rows, void* y,
+                    int y_dtype, uint64_t y_pitch, void* workspace, uint64_t workspace_bytes, uint32_t* fault_dev, void* stream, char* err,
+                    size_t errlen);
+
+/* The step between two blocks in one pass over each row [width] (1..32,768), m26b_rank_sum_residual_dev with the norms around it:
+ *   u = planes[0] + planes[1] + ...            rank order, FP32
+ *   u = u / sqrt(mean(u^2) + eps) * post_w     if post_w
+ *   h = residual_scale * residual + y_scale * gate * u
+ *   n = h / sqrt(mean(h^2) + eps) * pre_w      if n_out (pre_w NULL: a norm without weights)
+ * planes: a HOST array of n_planes device pointers (0..8; 0: no block output, then no post_w and no gate), rows y_pitch
+ * elements apart, y_dtype. residual / h_out: h_dtype, h_pitch; residual may be NULL (0) and may be h_out itself (in place).
+ * n_out: n_dtype, n_pitch. h_out or n_out may be NULL, not both. dtypes: 0 = BF16, 1 = FP32; a pitch of 0 means dense rows.
+ * gate_kind: 0 none; 1 one FP32 per token [rows]; 2 one per channel [width], w_dtype; 3 one per element, as a plane
+ * (y_dtype, y_pitch). post_w, pre_w [width]: w_dtype. eps > 0. FP32 throughout, one rounding per output; n is computed from h
+ * before h is rounded. A sum of squares beyond FP32 is rescaled, so finite rows have finite norms. Enqueued on `stream`
+ * (NULL = the default stream); outputs other than h_out == residual must not overlap inputs. 0 rows is no work. */
+int m26b_block_norm_dev(const void* const* planes, int n_planes, int y_dtype, uint64_t y_pitch, float y_scale, const void* post_w, const void* gate,
+                        int gate_kind, const void* residual, int h_dtype, uint64_t h_pitch, float residual_scale, const void* pre_w, int w_dtype,
+                        float eps, uint32_t rows, uint32_t width, void* h_out, void* n_out, int n_dtype, uint64_t n_pitch, void* stream, char* err,
+                        size_t errlen);
+
 /* Library identity: "m26b-expert <version> sm_100a". */
 const char* m26b_version(void);
 

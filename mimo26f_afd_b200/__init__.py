@@ -6,6 +6,15 @@ Rust wrapper (``crates/mimo26-spark/src/b1.rs``): ``Layer``, ``Scratch``, ``ffn`
 ``ffn_strided``, ``FfnStats``. There is no CPU path: importing the bindings without the
 built library raises.
 """
+from .dense import (  # noqa: F401
+    GATE_CHANNEL,
+    GATE_ELEMENT,
+    GATE_NONE,
+    GATE_TOKEN,
+    Linear,
+    block_norm_dev,
+    linear_dev,
+)
 from .expert import (  # noqa: F401
     Exchange,
     ExpertError,

@@ -23,6 +23,8 @@ SYMBOLS = (
     "m26b_ffn_tp", "m26b_ffn_tp_dev", "m26b_ep_ffn", "m26b_layer_image", "m26b_layer_new_from_checkpoint_ep_replicated",
     "m26b_frame_request_bytes", "m26b_frame_return_bytes", "m26b_frame_crc32c", "m26b_frame_crc32c_table", "m26b_frame_encode_request",
     "m26b_serve_frame", "m26b_frame_parse_return", "m26b_frame_check_request",
+    "m26b_linear_new", "m26b_linear_new_gated", "m26b_linear_free", "m26b_linear_workspace_bytes", "m26b_linear_dev",
+    "m26b_block_norm_dev",
 )
 
 _lib = None
@@ -64,6 +66,15 @@ def lib() -> C.CDLL:
     L.m26b_ep_set_route_output.argtypes = [vp, C.c_int]
     L.m26b_scratch_timings.argtypes = [vp, f32p, *err]
     L.m26b_scratch_peek.argtypes = [vp, C.c_int, vp, C.c_uint64, *err]
+    L.m26b_linear_new.argtypes = [u8p, u8p, C.c_uint32, C.c_uint32, C.POINTER(vp), *err]
+    L.m26b_linear_new_gated.argtypes = [u8p, u8p, u8p, u8p, C.c_uint32, C.c_uint32, C.POINTER(vp), *err]
+    L.m26b_linear_free.argtypes = [vp]
+    L.m26b_linear_free.restype = None
+    L.m26b_linear_workspace_bytes.argtypes = [vp, C.c_uint32]
+    L.m26b_linear_workspace_bytes.restype = C.c_uint64
+    L.m26b_linear_dev.argtypes = [vp, vp, C.c_int, u8p, C.c_uint64, C.c_uint32, vp, C.c_int, C.c_uint64, vp, C.c_uint64, u32p, vp, *err]
+    L.m26b_block_norm_dev.argtypes = [C.POINTER(vp), C.c_int, C.c_int, C.c_uint64, C.c_float, vp, vp, C.c_int, vp, C.c_int, C.c_uint64, C.c_float,
+                                      vp, C.c_int, C.c_float, C.c_uint32, C.c_uint32, vp, vp, C.c_int, C.c_uint64, vp, *err]
     L.m26b_quantize_dev.argtypes = [vp, C.c_int, C.c_uint64, C.c_int, u8p, u8p, u32p, vp, *err]
     L.m26b_route_reduce_dev.argtypes = [f32p, f32p, C.c_uint32, f32p, u16p, u32p, vp, *err]
     L.m26b_rank_sum_dev.argtypes = [C.POINTER(vp), C.c_int, C.c_uint64, f32p, vp, *err]

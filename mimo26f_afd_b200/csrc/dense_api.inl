@@ -1,0 +1,259 @@
+// C ABI of the dense operators around the routed experts: the MXFP4 linear / gated projections (linear_w4.cuh) and the step
+// between two blocks (block_norm.cuh). Included into the library's single translation unit behind m26b_api.cu's helpers.
+#pragma once
+#include <new>
+
+struct m26b_linear {
+    uint8_t *w = nullptr, *sf = nullptr;        // weight image (linear_w4.cuh)
+    uint32_t n = 0, k = 0, k_pad = 0;
+    bool gated = false;
+    int device = 0, sms = 0;
+    CUtensorMap map_w;
+};
+
+namespace {
+
+constexpr uint32_t kLinearMaxDim = 1u << 20;
+constexpr uint32_t kLinearPassRows = 8192;      // tokens per pass: bounds the workspace at 2 x 8192 x k bytes
+
+// The gated weight image [rows][k_pad] seen as [blocks of 128 rows][128][k_pad] (blocks alternate gate / up), boxes of 128 elements x
+// 64 rows x 2 blocks: one copy brings 64 gate rows and the 64 up rows of the same features.
+bool make_map_gated(CUtensorMap* m, void* base, uint64_t k_pad, uint64_t rows) {
+    EncodeTiledFn f = encode_fn();
+    if (!f) return false;
+    cuuint64_t dims[3] = {k_pad, uint64_t(kTileM), rows / kTileM};
+    cuuint64_t strides[2] = {k_pad / 2, uint64_t(kTileM) * (k_pad / 2)};
+    cuuint32_t box[3] = {128, kTileM / 2, 2};
+    cuuint32_t es[3] = {1, 1, 1};
+    return f(m, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 3, base, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool gated, uint32_t n, uint32_t k, m26b_linear** out, char* err,
+               size_t errlen) {
+    if (!out || !w[0] || !s[0] || (gated && (!w[1] || !s[1])) || !n || n > kLinearMaxDim || !k || k > kLinearMaxDim || k % kBlockK) {
+        set_msg(err, errlen, "m26b linear: bad tensors/extents (k a multiple of 32)");
+        return 1;
+    }
+    *out = nullptr;
+    m26b_linear* L = new (std::nothrow) m26b_linear;
+    if (!L) { set_msg(err, errlen, "m26b linear: out of host memory"); return 2; }
+    L->n = n; L->k = k; L->gated = gated;
+    L->k_pad = (k + kChunkK - 1) / kChunkK * kChunkK;
+    const uint64_t feats = gated ? kTileM : kPairM;                    // output features per 256 image rows
+    const uint64_t rows = (n + feats - 1) / feats * kPairM, chunks = L->k_pad / kChunkK;
+    const uint64_t w_bytes = rows * (L->k_pad / 2), sf_bytes = rows / kTileM * chunks * kScaleBlockBytes;
+    auto fail = [&](const char* what, cudaError_t e) {
+        set_err(err, errlen, what, e);
+        m26b_linear_free(L);
+        return 2;
+    };
+    cudaError_t e = cudaGetDevice(&L->device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&L->sms, cudaDevAttrMultiProcessorCount, L->device);
+    if (e != cudaSuccess) return fail("m26b linear device", e);
+    if ((e = cudaDeviceSynchronize()) != cudaSuccess) return fail("m26b linear sync", e);      // the source may come from any stream
+    void* mem = nullptr;
+    if ((e = cudaMalloc(&mem, w_bytes)) != cudaSuccess) return fail("m26b linear weights alloc", e);
+    L->w = static_cast<uint8_t*>(mem);
+    if ((e = cudaMalloc(&mem, sf_bytes)) != cudaSuccess) return fail("m26b linear scales alloc", e);
+    L->sf = static_cast<uint8_t*>(mem);
+    const LinearSrc src{{w[0], w[1]}, {s[0], s[1]}};
+    linear_prep_payload_kernel<<<L->sms * 8, 256>>>(src, gated, n, k, L->k_pad, rows, L->w);
+    linear_prep_scales_kernel<<<L->sms * 8, 256>>>(src, gated, n, k, uint32_t(chunks), sf_bytes, L->sf);
+    if ((e = cudaGetLastError()) != cudaSuccess) return fail("m26b linear prepare launch", e);
+    if ((e = cudaDeviceSynchronize()) != cudaSuccess) return fail("m26b linear prepare", e);
+    if (!(gated ? make_map_gated(&L->map_w, L->w, L->k_pad, rows) : make_map(&L->map_w, true, L->w, L->k_pad, rows, L->k_pad / 2, kTileM))) {
+        set_msg(err, errlen, "m26b linear: cuTensorMapEncodeTiled failed for the weights");
+        m26b_linear_free(L);
+        return 2;
+    }
+    *out = L;
+    return 0;
+}
+
+uint32_t linear_rows_cap(uint32_t rows) { return ((rows < kLinearPassRows ? rows : kLinearPassRows) + 15) & ~15u; }
+
+template <int B_ROWS, int PIECES, bool GATED>
+cudaError_t launch_linear(const m26b_linear* L, const TokenMaps& mx, const LinearArgs& a, cudaStream_t st) {
+    using T = LinearTile<B_ROWS, PIECES>;
+    const auto kernel = linear_w4_kernel<B_ROWS, PIECES, GATED>;
+    const int smem = int(sizeof(LinearSmem<B_ROWS, PIECES>)) + 1024;
+    static std::atomic<uint64_t> opted{0};                             // one flag bit per device of this process
+    const uint64_t bit = 1ull << (L->device & 63);
+    if (!(opted.load(std::memory_order_relaxed) & bit)) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        opted.fetch_or(bit, std::memory_order_relaxed);
+    }
+    const uint32_t tiles = GATED ? (a.n + 63) / 64 : (a.n + kTileM - 1) / kTileM, tok_tiles = (a.rows + B_ROWS - 1) / B_ROWS;
+    // K is split over a cluster while the CTAs still fit the SMs at once and each keeps at least two chunks
+    uint32_t split = 1;
+    while (split < 8 && uint64_t(tiles) * tok_tiles * split * 2 <= uint64_t(L->sms) * T::kCtasPerSm && a.chunks >= split * 4) split *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(tiles * split, tok_tiles); cfg.blockDim = dim3(kLinearThreads); cfg.dynamicSmemBytes = size_t(smem); cfg.stream = st;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = split; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, L->map_w, mx, a, split);
+}
+template <int B_ROWS>
+cudaError_t launch_linear_tile(const m26b_linear* L, bool bf16, const TokenMaps& mx, const LinearArgs& a, cudaStream_t st) {
+    if (L->gated) return bf16 ? launch_linear<B_ROWS, 2, true>(L, mx, a, st) : launch_linear<B_ROWS, 1, true>(L, mx, a, st);
+    return bf16 ? launch_linear<B_ROWS, 2, false>(L, mx, a, st) : launch_linear<B_ROWS, 1, false>(L, mx, a, st);
+}
+
+// One pass of at most kLinearPassRows tokens.
+int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x_scales, uint64_t x_pitch, uint32_t rows, void* y, int y_f32,
+                uint64_t y_pitch, uint8_t* ws, uint32_t* fault, cudaStream_t st, char* err, size_t errlen) {
+    const uint32_t pieces = bf16 ? 2 : 1, rows_cap = linear_rows_cap(rows);
+    uint8_t* sf = ws + uint64_t(pieces) * rows_cap * L->k_pad;
+    SplitArgs sp{x, x_scales, x_pitch, 0, rows, L->k, L->k_pad, rows_cap, ws, sf};
+    const uintptr_t xa = reinterpret_cast<uintptr_t>(x);
+    sp.vec = bf16 ? (xa % 16 == 0 && x_pitch % 8 == 0) : (xa % 8 == 0 && x_pitch % 8 == 0);
+    const uint64_t threads = uint64_t(rows) * (L->k_pad / 8);
+    const unsigned blocks = unsigned((threads + 255) / 256);
+    if (bf16) linear_split_kernel<2><<<blocks, 256, 0, st>>>(sp);
+    else linear_split_kernel<1><<<blocks, 256, 0, st>>>(sp);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) { set_err(err, errlen, "m26b linear stage launch", e); return 2; }
+    TokenMaps mx{};
+    for (int i = 0; i < 4; ++i)                     // the boxes a token tile of this request can use
+        if ((128u >> i) <= rows_cap && !make_map(&mx.box[i], false, ws, L->k_pad, uint64_t(pieces) * rows_cap, L->k_pad, 128u >> i)) {
+            set_msg(err, errlen, "m26b linear: cuTensorMapEncodeTiled failed for the activations");
+            return 2;
+        }
+    const LinearArgs a{L->sf, sf, rows, rows_cap, L->n, L->k_pad / kChunkK, y, y_f32, y_pitch, fault};
+    if (rows <= 16) e = launch_linear_tile<16>(L, bf16, mx, a, st);
+    else if (rows <= 32) e = launch_linear_tile<32>(L, bf16, mx, a, st);
+    else if (rows <= 64) e = launch_linear_tile<64>(L, bf16, mx, a, st);
+    else e = launch_linear_tile<128>(L, bf16, mx, a, st);
+    if (e != cudaSuccess) { cudaGetLastError(); set_err(err, errlen, "m26b linear launch", e); return 2; }
+    return 0;
+}
+
+template <int VEC, int PER>
+void launch_norm(const NormArgs& a, cudaStream_t st) {
+    const uint32_t threads = ((a.width + VEC * PER - 1) / (VEC * PER) + 31) & ~31u;
+    if (threads == 32) block_norm_kernel<VEC, PER, false><<<(a.rows + 3) / 4, 128, 0, st>>>(a);
+    else block_norm_kernel<VEC, PER, true><<<a.rows, threads, 0, st>>>(a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int m26b_linear_new(const uint8_t* w, const uint8_t* s, uint32_t n, uint32_t k, m26b_linear** out, char* err, size_t errlen) {
+    const uint8_t *ws[2] = {w, nullptr}, *ss[2] = {s, nullptr};
+    return linear_new(ws, ss, false, n, k, out, err, errlen);
+}
+int m26b_linear_new_gated(const uint8_t* gate_w, const uint8_t* gate_s, const uint8_t* up_w, const uint8_t* up_s, uint32_t n, uint32_t k,
+                          m26b_linear** out, char* err, size_t errlen) {
+    const uint8_t *ws[2] = {gate_w, up_w}, *ss[2] = {gate_s, up_s};
+    return linear_new(ws, ss, true, n, k, out, err, errlen);
+}
+void m26b_linear_free(m26b_linear* l) {
+    if (!l) return;
+    if (l->w) cudaFree(l->w);
+    if (l->sf) cudaFree(l->sf);
+    delete l;
+}
+uint64_t m26b_linear_workspace_bytes(const m26b_linear* l, uint32_t rows) {
+    if (!l || !rows) return 0;
+    const uint64_t cap = linear_rows_cap(rows);
+    return 2 * (cap * l->k_pad + (cap + 127) / 128 * (l->k_pad / kChunkK) * kScaleBlockBytes);
+}
+int m26b_linear_dev(const m26b_linear* l, const void* x, int x_dtype, const uint8_t* x_scales, uint64_t x_pitch, uint32_t rows, void* y,
+                    int y_dtype, uint64_t y_pitch, void* workspace, uint64_t workspace_bytes, uint32_t* fault_dev, void* stream, char* err,
+                    size_t errlen) {
+    if (!l || !(x_dtype == 0 || x_dtype == 2) || y_dtype < 0 || y_dtype > 1) {
+        set_msg(err, errlen, "m26b linear: bad handle/dtype (x 0 BF16 or 2 E4M3, y 0 BF16 or 1 FP32)");
+        return 1;
+    }
+    if (!rows) return 0;
+    if (!x_pitch) x_pitch = l->k;
+    if (!y_pitch) y_pitch = l->n;
+    if (!x || !y || !fault_dev || (x_dtype == 2 && !x_scales) || x_pitch < l->k || y_pitch < l->n) {
+        set_msg(err, errlen, "m26b linear: bad pointers/pitch");
+        return 1;
+    }
+    if ((x_dtype == 0 && reinterpret_cast<uintptr_t>(x) % 2) || reinterpret_cast<uintptr_t>(y) % (y_dtype ? 4 : 2)) {
+        set_msg(err, errlen, "m26b linear: x or y is not aligned to its element size");
+        return 1;
+    }
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 128 || workspace_bytes < m26b_linear_workspace_bytes(l, rows)) {
+        set_msg(err, errlen, "m26b linear: workspace too small or not 128-byte aligned (m26b_linear_workspace_bytes)");
+        return 1;
+    }
+    int dev = -1;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) { set_err(err, errlen, "m26b linear device", e); return 2; }
+    if (dev != l->device) { set_msg(err, errlen, "m26b linear: the handle belongs to another device"); return 1; }
+    const uint64_t x_row = x_pitch * (x_dtype == 0 ? 2 : 1), y_row = y_pitch * (y_dtype ? 4 : 2);
+    for (uint32_t r0 = 0; r0 < rows; r0 += kLinearPassRows) {
+        const uint32_t m = rows - r0 < kLinearPassRows ? rows - r0 : kLinearPassRows;
+        const int rc = linear_pass(l, static_cast<const uint8_t*>(x) + r0 * x_row, x_dtype == 0, x_scales ? x_scales + uint64_t(r0) * (l->k / kBlockK) : nullptr,
+                                   x_pitch, m, static_cast<uint8_t*>(y) + r0 * y_row, y_dtype, y_pitch, static_cast<uint8_t*>(workspace), fault_dev,
+                                   static_cast<cudaStream_t>(stream), err, errlen);
+        if (rc) return rc;
+    }
+    return 0;
+}
+
+int m26b_block_norm_dev(const void* const* planes, int n_planes, int y_dtype, uint64_t y_pitch, float y_scale, const void* post_w, const void* gate,
+                        int gate_kind, const void* residual, int h_dtype, uint64_t h_pitch, float residual_scale, const void* pre_w, int w_dtype,
+                        float eps, uint32_t rows, uint32_t width, void* h_out, void* n_out, int n_dtype, uint64_t n_pitch, void* stream, char* err,
+                        size_t errlen) {
+    const auto bad = [](int t) { return t < 0 || t > 1; };
+    if (n_planes < 0 || n_planes > 8 || (n_planes && !planes) || bad(y_dtype) || bad(h_dtype) || bad(w_dtype) || bad(n_dtype) || gate_kind < 0 ||
+        gate_kind > 3 || (gate_kind != 0) != (gate != nullptr) || (!n_planes && (post_w || gate)) || (!n_planes && !residual) || (!h_out && !n_out) ||
+        (!n_out && pre_w) || !width || width > kNormMaxWidth) {
+        set_msg(err, errlen, "m26b block norm: bad arguments");
+        return 1;
+    }
+    if (!(eps > 0.0f) || eps > 3.0e38f) { set_msg(err, errlen, "m26b block norm: eps must be positive"); return 1; }
+    if (!y_pitch) y_pitch = width;
+    if (!h_pitch) h_pitch = width;
+    if (!n_pitch) n_pitch = width;
+    if (y_pitch < width || h_pitch < width || n_pitch < width) { set_msg(err, errlen, "m26b block norm: a pitch is below the width"); return 1; }
+    NormArgs a{};
+    uintptr_t vec = 0, elem = 0;                      // address bits that keep 16-byte vectors / single elements from being aligned
+    const auto see = [&](const void* p, int f32) {
+        const uintptr_t v = reinterpret_cast<uintptr_t>(p);
+        vec |= v & 15; elem |= v & (f32 ? 3 : 1);
+    };
+    for (int r = 0; r < n_planes; ++r) {
+        if (!planes[r]) { set_msg(err, errlen, "m26b block norm: bad arguments"); return 1; }
+        a.y[r] = planes[r];
+        see(planes[r], y_dtype);
+    }
+    a.planes = n_planes;
+    a.y_f32 = y_dtype; a.h_f32 = h_dtype; a.n_f32 = n_dtype; a.w_f32 = w_dtype;
+    a.y_pitch = y_pitch; a.h_pitch = h_pitch; a.n_pitch = n_pitch;
+    a.post_w = post_w; a.gate = gate; a.residual = residual; a.pre_w = pre_w;
+    a.gate_kind = gate_kind;
+    a.y_scale = y_scale; a.residual_scale = residual_scale; a.eps = eps;
+    a.rows = rows; a.width = width; a.h_out = h_out; a.n_out = n_out;
+    see(post_w, w_dtype); see(pre_w, w_dtype); see(residual, h_dtype); see(h_out, h_dtype); see(n_out, n_dtype);
+    if (gate_kind == kGateToken) elem |= reinterpret_cast<uintptr_t>(gate) & 3;
+    else see(gate, gate_kind == kGateChannel ? w_dtype : y_dtype);
+    if (elem) { set_msg(err, errlen, "m26b block norm: a pointer is not aligned to its element size"); return 1; }
+    if (!rows) return 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!vec && (width | (n_planes ? y_pitch : 0) | (residual || h_out ? h_pitch : 0) | (n_out ? n_pitch : 0)) % 8 == 0) {
+        if (width <= 8192) launch_norm<8, 1>(a, st);
+        else if (width <= 16384) launch_norm<8, 2>(a, st);
+        else launch_norm<8, 4>(a, st);
+    } else {
+        if (width <= 4096) launch_norm<1, 4>(a, st);
+        else if (width <= 16384) launch_norm<1, 16>(a, st);
+        else launch_norm<1, 32>(a, st);
+    }
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) { set_err(err, errlen, "m26b block norm launch", e); return 2; }
+    return 0;
+}
+
+}  // extern "C"

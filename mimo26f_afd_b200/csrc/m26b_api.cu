@@ -17,6 +17,8 @@
 #include "gemm_mx_pair.cuh"
 #include "prologue_small.cuh"
 #include "ep_kernels.cuh"
+#include "block_norm.cuh"
+#include "linear_w4.cuh"
 #include "frame.inl"
 
 using namespace m26b;
@@ -1956,3 +1958,5 @@ int m26b_scratch_peek(m26b_scratch* S, int what, void* host_dst, uint64_t bytes,
 }
 
 }  // extern "C"
+
+#include "dense_api.inl"

@@ -1,0 +1,86 @@
+"""Dense operators around the routed experts, over the C ABI: projections with MXFP4 weights in the checkpoint layout (a
+shared expert, a first dense layer) and the step between two blocks (rank sum, norms, gate, residual).
+
+Where the reference has cuBLAS projections on the coordinator (crates/mimo26-coordinator/src/gpu_dense.rs) and separate
+launches for the rank sum, the residual add and the norm (kernels/glue.cu), these work on the expert weights' own format and
+in one pass. Arguments are device buffers (anything with ``data_ptr()`` or an address); work is enqueued on ``stream`` (an
+address; None = the default stream) and nothing is synchronised.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _native
+from .expert import X_BF16, ExpertError, _check, _ptr
+
+GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_ELEMENT = 0, 1, 2, 3
+Y_BF16, Y_F32 = 0, 1
+
+
+class Linear:
+    """One prepared MXFP4 matrix (``new``: y = x W^T) or gated pair (``gated``: silu(x Wg^T) * (x Wu^T)) on the current
+    device. Weights ``w`` u8 [n, k/2], scales ``s`` u8 [n, k/32]; the sources may be freed afterwards."""
+
+    def __init__(self, handle: int, n: int, k: int):
+        self._h, self.n, self.k = C.c_void_p(handle), n, k
+
+    @classmethod
+    def new(cls, w, s, n: int, k: int) -> "Linear":
+        out, err = C.c_void_p(), C.create_string_buffer(256)
+        _check(_native.lib().m26b_linear_new(_ptr(w), _ptr(s), n, k, C.byref(out), err, 256), err)
+        return cls(out.value, n, k)
+
+    @classmethod
+    def gated(cls, gate_w, gate_s, up_w, up_s, n: int, k: int) -> "Linear":
+        out, err = C.c_void_p(), C.create_string_buffer(256)
+        _check(_native.lib().m26b_linear_new_gated(_ptr(gate_w), _ptr(gate_s), _ptr(up_w), _ptr(up_s), n, k, C.byref(out), err, 256), err)
+        return cls(out.value, n, k)
+
+    def workspace_bytes(self, rows: int) -> int:
+        """Device bytes ``linear_dev`` needs for ``rows`` tokens."""
+        return int(_native.lib().m26b_linear_workspace_bytes(self._h, rows))
+
+    def close(self) -> None:
+        if self._h:
+            _native.lib().m26b_linear_free(self._h)
+            self._h = C.c_void_p(0)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _nbytes(buf) -> int:
+    n = getattr(buf, "nbytes", None)
+    if n is None:
+        raise ExpertError(1, "m26b linear: pass workspace_bytes with a workspace address")
+    return int(n)
+
+
+def linear_dev(layer: Linear, x, rows: int, y, *, x_dtype: int = X_BF16, x_scales=None, x_pitch: int = 0, y_dtype: int = Y_BF16,
+               y_pitch: int = 0, workspace=None, workspace_bytes=None, fault=None, stream=None) -> None:
+    """y [rows, n] from x [rows, k] (BF16, or E4M3 with ``x_scales`` [rows, k/32]); pitches in elements, 0 = dense rows.
+    ``workspace`` holds ``layer.workspace_bytes(rows)`` bytes and serves one call at a time; ``fault`` is one int32 / uint32
+    that receives code 3 if a bounded wait inside the kernel ran out."""
+    if workspace_bytes is None:
+        workspace_bytes = 0 if workspace is None else _nbytes(workspace)
+    err = C.create_string_buffer(256)
+    rc = _native.lib().m26b_linear_dev(layer._h, _ptr(x), x_dtype, _ptr(x_scales), x_pitch, rows, _ptr(y), y_dtype, y_pitch, _ptr(workspace),
+                                       workspace_bytes, _ptr(fault), _ptr(stream), err, 256)
+    _check(rc, err)
+
+
+def block_norm_dev(planes, residual, rows: int, width: int, *, post_w=None, gate=None, gate_kind: int = GATE_NONE, y_dtype: int = 0,
+                   y_pitch: int = 0, y_scale: float = 1.0, h_dtype: int = 1, h_pitch: int = 0, residual_scale: float = 1.0, pre_w=None,
+                   w_dtype: int = 1, eps: float = 1e-6, h_out=None, n_out=None, n_dtype: int = 0, n_pitch: int = 0, stream=None) -> None:
+    """u = sum of ``planes`` in order, normed with ``post_w`` if given; h = residual_scale * residual + y_scale * gate * u into
+    ``h_out``; n = the RMS norm of h (times ``pre_w``) into ``n_out``. dtypes 0 = BF16, 1 = FP32; pitches in elements, 0 =
+    dense rows; ``planes`` a sequence of up to eight device buffers (empty: norm of the residual alone)."""
+    arr = (C.c_void_p * max(1, len(planes)))(*[_ptr(p) for p in planes])
+    err = C.create_string_buffer(256)
+    rc = _native.lib().m26b_block_norm_dev(arr, len(planes), y_dtype, y_pitch, y_scale, _ptr(post_w), _ptr(gate), gate_kind, _ptr(residual), h_dtype,
+                                           h_pitch, residual_scale, _ptr(pre_w), w_dtype, eps, rows, width, _ptr(h_out), _ptr(n_out), n_dtype,
+                                           n_pitch, _ptr(stream), err, 256)
+    _check(rc, err)
