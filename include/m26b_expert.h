@@ -383,17 +383,28 @@ int m26b_linear_dev(const m26b_linear* l, const void* x, int x_dtype, const uint
  *   u = u / sqrt(mean(u^2) + eps) * post_w     if post_w
  *   h = residual_scale * residual + y_scale * gate * u
  *   n = h / sqrt(mean(h^2) + eps) * pre_w      if n_out (pre_w NULL: a norm without weights)
- * planes: a HOST array of n_planes device pointers (0..8; 0: no block output, then no post_w and no gate), rows y_pitch
- * elements apart, y_dtype. residual / h_out: h_dtype, h_pitch; residual may be NULL (0) and may be h_out itself (in place).
- * n_out: n_dtype, n_pitch. h_out or n_out may be NULL, not both. dtypes: 0 = BF16, 1 = FP32; a pitch of 0 means dense rows.
- * gate_kind: 0 none; 1 one FP32 per token [rows]; 2 one per channel [width], w_dtype; 3 one per element, as a plane
- * (y_dtype, y_pitch). post_w, pre_w [width]: w_dtype. eps > 0. FP32 throughout, one rounding per output; n is computed from h
- * before h is rounded. A sum of squares beyond FP32 is rescaled, so finite rows have finite norms. Enqueued on `stream`
- * (NULL = the default stream); outputs other than h_out == residual must not overlap inputs. 0 rows is no work. */
-int m26b_block_norm_dev(const void* const* planes, int n_planes, int y_dtype, uint64_t y_pitch, float y_scale, const void* post_w, const void* gate,
-                        int gate_kind, const void* residual, int h_dtype, uint64_t h_pitch, float residual_scale, const void* pre_w, int w_dtype,
-                        float eps, uint32_t rows, uint32_t width, void* h_out, void* n_out, int n_dtype, uint64_t n_pitch, void* stream, char* err,
-                        size_t errlen);
+ * dtypes: 0 = BF16, 1 = FP32; pitches are in elements, 0 means dense rows. FP32 throughout, one rounding per output; n is
+ * computed from h before h is rounded. A sum of squares beyond FP32 is rescaled, so finite rows have finite norms. The
+ * argument record is read before the call returns. Enqueued on `stream` (NULL = the default stream); outputs other than
+ * h_out == residual must not overlap inputs. 0 rows is no work. */
+typedef struct m26b_block_norm_args {
+    const void* planes[8];      /* device, the block's output: one plane per rank [rows][width], y_dtype, y_pitch */
+    const void* post_w;         /* [width] of w_dtype, or NULL: no norm of u */
+    const void* gate;           /* by gate_kind; NULL for kind 0 */
+    const void* residual;       /* [rows][width] of h_dtype, h_pitch, or NULL (0); may be h_out itself (in place) */
+    const void* pre_w;          /* [width] of w_dtype, or NULL */
+    void* h_out;                /* [rows][width] of h_dtype, h_pitch, or NULL */
+    void* n_out;                /* [rows][width] of n_dtype, n_pitch, or NULL; not both outputs NULL */
+    uint64_t y_pitch, h_pitch, n_pitch;
+    float y_scale, residual_scale;
+    float eps;                  /* > 0 */
+    uint32_t rows, width;
+    int32_t n_planes;           /* 0..8; 0: no block output, then no post_w and no gate */
+    int32_t gate_kind;          /* 0 none; 1 one FP32 per token [rows]; 2 one per channel [width], w_dtype; 3 one per element, as a plane */
+    int32_t y_dtype, h_dtype, n_dtype, w_dtype;
+    int32_t reserved;           /* 0 */
+} m26b_block_norm_args;
+int m26b_block_norm_dev(const m26b_block_norm_args* args, void* stream, char* err, size_t errlen);
 
 /* Library identity: "m26b-expert <version> sm_100a". */
 const char* m26b_version(void);

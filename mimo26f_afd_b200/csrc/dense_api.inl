@@ -202,21 +202,20 @@ int m26b_linear_dev(const m26b_linear* l, const void* x, int x_dtype, const uint
     return 0;
 }
 
-int m26b_block_norm_dev(const void* const* planes, int n_planes, int y_dtype, uint64_t y_pitch, float y_scale, const void* post_w, const void* gate,
-                        int gate_kind, const void* residual, int h_dtype, uint64_t h_pitch, float residual_scale, const void* pre_w, int w_dtype,
-                        float eps, uint32_t rows, uint32_t width, void* h_out, void* n_out, int n_dtype, uint64_t n_pitch, void* stream, char* err,
-                        size_t errlen) {
+int m26b_block_norm_dev(const m26b_block_norm_args* args, void* stream, char* err, size_t errlen) {
+    if (!args) { set_msg(err, errlen, "m26b block norm: bad arguments"); return 1; }
+    const m26b_block_norm_args& in = *args;
+    const int n_planes = in.n_planes, y_dtype = in.y_dtype, h_dtype = in.h_dtype, n_dtype = in.n_dtype, w_dtype = in.w_dtype, gate_kind = in.gate_kind;
+    const uint32_t rows = in.rows, width = in.width;
     const auto bad = [](int t) { return t < 0 || t > 1; };
-    if (n_planes < 0 || n_planes > 8 || (n_planes && !planes) || bad(y_dtype) || bad(h_dtype) || bad(w_dtype) || bad(n_dtype) || gate_kind < 0 ||
-        gate_kind > 3 || (gate_kind != 0) != (gate != nullptr) || (!n_planes && (post_w || gate)) || (!n_planes && !residual) || (!h_out && !n_out) ||
-        (!n_out && pre_w) || !width || width > kNormMaxWidth) {
+    if (n_planes < 0 || n_planes > 8 || bad(y_dtype) || bad(h_dtype) || bad(w_dtype) || bad(n_dtype) || gate_kind < 0 || gate_kind > 3 || in.reserved ||
+        (gate_kind != 0) != (in.gate != nullptr) || (!n_planes && (in.post_w || in.gate || !in.residual)) || (!in.h_out && !in.n_out) ||
+        (!in.n_out && in.pre_w) || !width || width > kNormMaxWidth) {
         set_msg(err, errlen, "m26b block norm: bad arguments");
         return 1;
     }
-    if (!(eps > 0.0f) || eps > 3.0e38f) { set_msg(err, errlen, "m26b block norm: eps must be positive"); return 1; }
-    if (!y_pitch) y_pitch = width;
-    if (!h_pitch) h_pitch = width;
-    if (!n_pitch) n_pitch = width;
+    if (!(in.eps > 0.0f) || in.eps > 3.0e38f) { set_msg(err, errlen, "m26b block norm: eps must be positive"); return 1; }
+    const uint64_t y_pitch = in.y_pitch ? in.y_pitch : width, h_pitch = in.h_pitch ? in.h_pitch : width, n_pitch = in.n_pitch ? in.n_pitch : width;
     if (y_pitch < width || h_pitch < width || n_pitch < width) { set_msg(err, errlen, "m26b block norm: a pitch is below the width"); return 1; }
     NormArgs a{};
     uintptr_t vec = 0, elem = 0;                      // address bits that keep 16-byte vectors / single elements from being aligned
@@ -225,24 +224,24 @@ int m26b_block_norm_dev(const void* const* planes, int n_planes, int y_dtype, ui
         vec |= v & 15; elem |= v & (f32 ? 3 : 1);
     };
     for (int r = 0; r < n_planes; ++r) {
-        if (!planes[r]) { set_msg(err, errlen, "m26b block norm: bad arguments"); return 1; }
-        a.y[r] = planes[r];
-        see(planes[r], y_dtype);
+        if (!in.planes[r]) { set_msg(err, errlen, "m26b block norm: bad arguments"); return 1; }
+        a.y[r] = in.planes[r];
+        see(in.planes[r], y_dtype);
     }
     a.planes = n_planes;
     a.y_f32 = y_dtype; a.h_f32 = h_dtype; a.n_f32 = n_dtype; a.w_f32 = w_dtype;
     a.y_pitch = y_pitch; a.h_pitch = h_pitch; a.n_pitch = n_pitch;
-    a.post_w = post_w; a.gate = gate; a.residual = residual; a.pre_w = pre_w;
+    a.post_w = in.post_w; a.gate = in.gate; a.residual = in.residual; a.pre_w = in.pre_w;
     a.gate_kind = gate_kind;
-    a.y_scale = y_scale; a.residual_scale = residual_scale; a.eps = eps;
-    a.rows = rows; a.width = width; a.h_out = h_out; a.n_out = n_out;
-    see(post_w, w_dtype); see(pre_w, w_dtype); see(residual, h_dtype); see(h_out, h_dtype); see(n_out, n_dtype);
-    if (gate_kind == kGateToken) elem |= reinterpret_cast<uintptr_t>(gate) & 3;
-    else see(gate, gate_kind == kGateChannel ? w_dtype : y_dtype);
+    a.y_scale = in.y_scale; a.residual_scale = in.residual_scale; a.eps = in.eps;
+    a.rows = rows; a.width = width; a.h_out = in.h_out; a.n_out = in.n_out;
+    see(in.post_w, w_dtype); see(in.pre_w, w_dtype); see(in.residual, h_dtype); see(in.h_out, h_dtype); see(in.n_out, n_dtype);
+    if (gate_kind == kGateToken) elem |= reinterpret_cast<uintptr_t>(in.gate) & 3;
+    else see(in.gate, gate_kind == kGateChannel ? w_dtype : y_dtype);
     if (elem) { set_msg(err, errlen, "m26b block norm: a pointer is not aligned to its element size"); return 1; }
     if (!rows) return 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!vec && (width | (n_planes ? y_pitch : 0) | (residual || h_out ? h_pitch : 0) | (n_out ? n_pitch : 0)) % 8 == 0) {
+    if (!vec && (width | (n_planes ? y_pitch : 0) | (in.residual || in.h_out ? h_pitch : 0) | (in.n_out ? n_pitch : 0)) % 8 == 0) {
         if (width <= 8192) launch_norm<8, 1>(a, st);
         else if (width <= 16384) launch_norm<8, 2>(a, st);
         else launch_norm<8, 4>(a, st);

@@ -9,12 +9,39 @@ address; None = the default stream) and nothing is synchronised.
 from __future__ import annotations
 
 import ctypes as C
+import struct
+import threading
 
 from . import _native
 from .expert import X_BF16, ExpertError, _check, _ptr
 
 GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_ELEMENT = 0, 1, 2, 3
 Y_BF16, Y_F32 = 0, 1
+
+
+# struct m26b_block_norm_args of the header
+_NORM_ARGS = struct.Struct("@14P3Q3f2I7i")
+_local = threading.local()
+
+
+def _err():
+    """This thread's error buffer (a decode step makes several calls per layer; a fresh buffer each costs more than the check)."""
+    try:
+        return _local.err
+    except AttributeError:
+        _local.err = C.create_string_buffer(256)
+        return _local.err
+
+
+def _addr(x) -> int:
+    if x is None:
+        return 0
+    if type(x) is int:
+        return x
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return _ptr(x)
 
 
 class Linear:
@@ -66,10 +93,11 @@ def linear_dev(layer: Linear, x, rows: int, y, *, x_dtype: int = X_BF16, x_scale
     that receives code 3 if a bounded wait inside the kernel ran out."""
     if workspace_bytes is None:
         workspace_bytes = 0 if workspace is None else _nbytes(workspace)
-    err = C.create_string_buffer(256)
-    rc = _native.lib().m26b_linear_dev(layer._h, _ptr(x), x_dtype, _ptr(x_scales), x_pitch, rows, _ptr(y), y_dtype, y_pitch, _ptr(workspace),
-                                       workspace_bytes, _ptr(fault), _ptr(stream), err, 256)
-    _check(rc, err)
+    err = _err()
+    rc = _native.lib().m26b_linear_dev(layer._h, _addr(x), x_dtype, _addr(x_scales), x_pitch, rows, _addr(y), y_dtype, y_pitch, _addr(workspace),
+                                       workspace_bytes, _addr(fault), _addr(stream), err, 256)
+    if rc:
+        _check(rc, err)
 
 
 def block_norm_dev(planes, residual, rows: int, width: int, *, post_w=None, gate=None, gate_kind: int = GATE_NONE, y_dtype: int = 0,
@@ -78,9 +106,19 @@ def block_norm_dev(planes, residual, rows: int, width: int, *, post_w=None, gate
     """u = sum of ``planes`` in order, normed with ``post_w`` if given; h = residual_scale * residual + y_scale * gate * u into
     ``h_out``; n = the RMS norm of h (times ``pre_w``) into ``n_out``. dtypes 0 = BF16, 1 = FP32; pitches in elements, 0 =
     dense rows; ``planes`` a sequence of up to eight device buffers (empty: norm of the residual alone)."""
-    arr = (C.c_void_p * max(1, len(planes)))(*[_ptr(p) for p in planes])
-    err = C.create_string_buffer(256)
-    rc = _native.lib().m26b_block_norm_dev(arr, len(planes), y_dtype, y_pitch, y_scale, _ptr(post_w), _ptr(gate), gate_kind, _ptr(residual), h_dtype,
-                                           h_pitch, residual_scale, _ptr(pre_w), w_dtype, eps, rows, width, _ptr(h_out), _ptr(n_out), n_dtype,
-                                           n_pitch, _ptr(stream), err, 256)
-    _check(rc, err)
+    n = len(planes)
+    if n > 8:
+        raise ExpertError(1, "m26b block norm: bad arguments")
+    try:
+        args = _NORM_ARGS.pack(*[_addr(p) for p in planes], *_PAD[n], _addr(post_w), _addr(gate), _addr(residual), _addr(pre_w), _addr(h_out),
+                               _addr(n_out), y_pitch, h_pitch, n_pitch, y_scale, residual_scale, eps, rows, width, n, gate_kind, y_dtype, h_dtype,
+                               n_dtype, w_dtype, 0)
+    except (struct.error, OverflowError) as e:        # a negative or oversized number
+        raise ExpertError(1, f"m26b block norm: bad arguments ({e})") from None
+    err = _err()
+    rc = _native.lib().m26b_block_norm_dev(args, _addr(stream), err, 256)
+    if rc:
+        _check(rc, err)
+
+
+_PAD = [(0,) * (8 - i) for i in range(9)]
