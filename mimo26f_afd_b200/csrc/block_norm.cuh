@@ -25,7 +25,7 @@ struct NormArgs {
     uint64_t y_pitch, h_pitch, n_pitch;     // elements
     const void *post_w, *gate, *residual, *pre_w;
     int gate_kind;
-    float y_scale, residual_scale, eps;
+    float y_scale, residual_scale, eps, inv_width;      // y_scale 0 without planes, residual_scale 0 without a residual
     uint32_t rows, width;
     void *h_out, *n_out;
 };
@@ -89,7 +89,7 @@ __device__ __forceinline__ float row_reduce(float v, float* slots) {
 // 1 / sqrt(mean(v^2) + eps) over the row. A sum of squares that leaves FP32 (values above 2^63) is taken again of the
 // row divided by a power of two near its largest magnitude; rows that hold an infinity or a NaN keep what FP32 gives.
 template <int E, bool BLOCK>
-__device__ __forceinline__ float row_rrms(const float (&v)[E], uint32_t width, float eps, float (*slots)[32]) {
+__device__ __forceinline__ float row_rrms(const float (&v)[E], float inv_width, float eps, float (*slots)[32]) {
     float ss = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) ss = fmaf(v[e], v[e], ss);
@@ -105,92 +105,140 @@ __device__ __forceinline__ float row_rrms(const float (&v)[E], uint32_t width, f
 #pragma unroll
             for (int e = 0; e < E; ++e) { const float a = v[e] * down; s2 = fmaf(a, a, s2); }
             s2 = row_reduce<OpSum, BLOCK>(s2, slots[2]);
-            return down / sqrtf(s2 / float(width));                      // eps * 2^-200 is nothing beside s2 >= 2^-74
+            return down * rsqrtf(s2 * inv_width);                        // eps * 2^-200 is nothing beside s2 >= 2^-74
         }
     }
-    return 1.0f / sqrtf(ss / float(width) + eps);
+    return rsqrtf(fmaf(ss, inv_width, eps));
 }
 
-// One row per warp (BLOCK false, blockDim / 32 rows per CTA) or per CTA.
-template <int VEC, int PER, bool BLOCK>
-__global__ void __launch_bounds__(1024) block_norm_kernel(const NormArgs p) {
-    __shared__ float slots[6][32];
+// VEC elements as they lie in memory: loads are issued for a whole row before anything waits for one of them.
+template <int VEC, bool F32>
+struct RawVec {
+    uint32_t w[VEC == 1 ? 1 : VEC * (F32 ? 4 : 2) / 4];
+    __device__ __forceinline__ void load(const void* base, uint64_t i) {
+        if constexpr (VEC == 1) {
+            if constexpr (F32) w[0] = static_cast<const uint32_t*>(base)[i];
+            else w[0] = static_cast<const uint16_t*>(base)[i];
+        } else {
+            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + i * (F32 ? 4 : 2));
+#pragma unroll
+            for (int q = 0; q < VEC * (F32 ? 4 : 2) / 16; ++q) { const uint4 a = p[q]; w[4 * q] = a.x; w[4 * q + 1] = a.y; w[4 * q + 2] = a.z; w[4 * q + 3] = a.w; }
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (uint32_t& v : w) v = 0;
+    }
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (F32) return __uint_as_float(w[e]);
+        else return __uint_as_float((e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+};
+
+// A row belongs to a warp (MAX_THREADS 128: four rows per CTA) or to a CTA; both stride over the rows by the grid, and the
+// next row's operands are requested before this row's reductions are waited for. Y32 / H32: FP32 planes / residual stream.
+template <int VEC, int PER, int MAX_THREADS, bool Y32, bool H32>
+__global__ void __launch_bounds__(MAX_THREADS) block_norm_kernel(const NormArgs p) {
+    constexpr bool BLOCK = MAX_THREADS > 128;
+    __shared__ float slots_all[2][6][32];
     const uint32_t threads = BLOCK ? blockDim.x : 32u;
     const uint32_t t = BLOCK ? threadIdx.x : threadIdx.x & 31u;
-    const uint32_t row = BLOCK ? blockIdx.x : blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (row >= p.rows) return;                       // whole warps; never taken when the CTA shares a row
-    const uint64_t yo = uint64_t(row) * p.y_pitch, ho = uint64_t(row) * p.h_pitch, no = uint64_t(row) * p.n_pitch;
-    float u[PER * VEC], h[PER * VEC];
+    const uint32_t rows_at_once = BLOCK ? gridDim.x : gridDim.x * (blockDim.x >> 5);
+    uint32_t row = BLOCK ? blockIdx.x : blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    RawVec<VEC, Y32> ry[PER], rg[PER];
+    RawVec<VEC, H32> rh[PER];
+    const bool has_y = p.planes > 0, has_h = p.residual != nullptr, gate_elem = p.gate_kind == kGateElement;
+    const auto request = [&](uint32_t r) {
+        const uint64_t yo = uint64_t(r) * p.y_pitch, ho = uint64_t(r) * p.h_pitch;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const uint32_t i = (t + j * threads) * VEC;
-        float a[VEC], r[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) { a[e] = 0.0f; r[e] = 0.0f; }
-        if (i < p.width) {
-            if (p.planes) load_elems<VEC>(p.y[0], p.y_f32, yo + i, a);
-            if (p.residual) load_elems<VEC>(p.residual, p.h_f32, ho + i, r);
-#pragma unroll
-            for (int q = 1; q < 8; ++q) {
-                if (q >= p.planes) break;
-                float b[VEC];
-                load_elems<VEC>(p.y[q], p.y_f32, yo + i, b);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) a[e] += b[e];
+        for (int j = 0; j < PER; ++j) {
+            const uint32_t i = (t + j * threads) * VEC;
+            if (i < p.width) {
+                if (has_y) ry[j].load(p.y[0], yo + i);
+                if (has_h) rh[j].load(p.residual, ho + i);
+                if (gate_elem) rg[j].load(p.gate, yo + i);
             }
         }
+    };
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) { u[j * VEC + e] = a[e]; h[j * VEC + e] = r[e]; }
-    }
-    const float r1 = p.post_w ? row_rrms<PER * VEC, BLOCK>(u, p.width, p.eps, slots) : 1.0f;
-    const float token_gate = p.gate_kind == kGateToken ? static_cast<const float*>(p.gate)[row] : 1.0f;
+    for (int j = 0; j < PER; ++j) { ry[j].zero(); rh[j].zero(); rg[j].zero(); }
+    if (row < p.rows) request(row);
+    for (uint32_t turn = 0; row < p.rows; row += rows_at_once, ++turn) {
+        float (*slots)[32] = slots_all[turn & 1];    // the other set may still be read by slower warps of the row before
+        const uint64_t yo = uint64_t(row) * p.y_pitch, ho = uint64_t(row) * p.h_pitch, no = uint64_t(row) * p.n_pitch;
+        float u[PER * VEC], h[PER * VEC];
+        RawVec<VEC, Y32> cg[PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const uint32_t i = (t + j * threads) * VEC;
-        if (i >= p.width) continue;
-        float a[VEC], w[VEC];
+        for (int j = 0; j < PER; ++j) {
+            cg[j] = rg[j];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) a[e] = h[j * VEC + e] * p.residual_scale;
-        if (p.planes) {
-            float b[VEC];
+            for (int e = 0; e < VEC; ++e) { u[j * VEC + e] = ry[j].get(e); h[j * VEC + e] = rh[j].get(e); }
+        }
+        if (p.planes > 1) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) b[e] = u[j * VEC + e];
+            for (int j = 0; j < PER; ++j) {
+                const uint32_t i = (t + j * threads) * VEC;
+                if (i >= p.width) continue;
+                RawVec<VEC, Y32> more[7];
+#pragma unroll
+                for (int q = 0; q < 7; ++q) {
+                    more[q].zero();
+                    if (q + 1 < p.planes) more[q].load(p.y[q + 1], yo + i);
+                }
+#pragma unroll
+                for (int q = 0; q < 7; ++q) {
+                    if (q + 1 >= p.planes) break;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) u[j * VEC + e] += more[q].get(e);
+                }
+            }
+        }
+        if (rows_at_once < p.rows - row) request(row + rows_at_once);
+        float r1 = p.y_scale;                          // every factor of u that the row shares
+        if (p.gate_kind == kGateToken) r1 *= static_cast<const float*>(p.gate)[row];
+        if (p.post_w) r1 *= row_rrms<PER * VEC, BLOCK>(u, p.inv_width, p.eps, slots);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const uint32_t i = (t + j * threads) * VEC;
+            if (i >= p.width) continue;
+            float a[VEC], w[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[e] = u[j * VEC + e] * r1;
             if (p.post_w) {
                 load_elems<VEC>(p.post_w, p.w_f32, i, w);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) b[e] = b[e] * r1 * w[e];
+                for (int e = 0; e < VEC; ++e) a[e] *= w[e];
             }
-            if (p.gate_kind >= kGateChannel) {
-                if (p.gate_kind == kGateChannel) load_elems<VEC>(p.gate, p.w_f32, i, w);
-                else load_elems<VEC>(p.gate, p.y_f32, yo + i, w);
+            if (gate_elem) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) b[e] *= w[e];
+                for (int e = 0; e < VEC; ++e) a[e] *= cg[j].get(e);
+            } else if (p.gate_kind == kGateChannel) {
+                load_elems<VEC>(p.gate, p.w_f32, i, w);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) a[e] *= w[e];
             }
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float g = p.y_scale * (b[e] * token_gate);
-                a[e] = p.residual ? fmaf(h[j * VEC + e], p.residual_scale, g) : g;
-            }
+            for (int e = 0; e < VEC; ++e) a[e] = fmaf(h[j * VEC + e], p.residual_scale, a[e]);
+            if (p.h_out) store_elems<VEC>(p.h_out, H32, ho + i, a);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) h[j * VEC + e] = a[e];
         }
-        if (p.h_out) store_elems<VEC>(p.h_out, p.h_f32, ho + i, a);
+        if (!p.n_out) continue;
+        const float r2 = row_rrms<PER * VEC, BLOCK>(h, p.inv_width, p.eps, slots + 3);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) h[j * VEC + e] = a[e];
-    }
-    if (!p.n_out) return;
-    const float r2 = row_rrms<PER * VEC, BLOCK>(h, p.width, p.eps, slots + 3);
+        for (int j = 0; j < PER; ++j) {
+            const uint32_t i = (t + j * threads) * VEC;
+            if (i >= p.width) continue;
+            float a[VEC], w[VEC];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const uint32_t i = (t + j * threads) * VEC;
-        if (i >= p.width) continue;
-        float a[VEC], w[VEC];
+            for (int e = 0; e < VEC; ++e) a[e] = h[j * VEC + e] * r2;
+            if (p.pre_w) {
+                load_elems<VEC>(p.pre_w, p.w_f32, i, w);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) a[e] = h[j * VEC + e] * r2;
-        if (p.pre_w) {
-            load_elems<VEC>(p.pre_w, p.w_f32, i, w);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) a[e] *= w[e];
+                for (int e = 0; e < VEC; ++e) a[e] *= w[e];
+            }
+            store_elems<VEC>(p.n_out, p.n_f32, no + i, a);
         }
-        store_elems<VEC>(p.n_out, p.n_f32, no + i, a);
     }
 }
 

@@ -134,11 +134,32 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
     return 0;
 }
 
-template <int VEC, int PER>
-void launch_norm(const NormArgs& a, cudaStream_t st) {
+// Rows are strided over by as many CTAs as the GPU holds at once.
+template <int VEC, int PER, int MAX_THREADS, bool Y32, bool H32>
+cudaError_t launch_norm_kernel(const NormArgs& a, uint32_t threads, cudaStream_t st) {
+    const auto kernel = block_norm_kernel<VEC, PER, MAX_THREADS, Y32, H32>;
+    static const int sms = [] { int dev = 0, n = 148; cudaGetDevice(&dev); cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev); return n; }();
+    static std::atomic<int> resident[33]{};                            // CTAs per SM by warps per CTA
+    const uint32_t block = MAX_THREADS == 128 ? 128u : threads;
+    int per_sm = resident[block / 32].load(std::memory_order_relaxed);
+    if (!per_sm) {
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, int(block), 0);
+        if (e != cudaSuccess || per_sm < 1) return e != cudaSuccess ? e : cudaErrorLaunchOutOfResources;
+        resident[block / 32].store(per_sm, std::memory_order_relaxed);
+    }
+    const uint32_t need = MAX_THREADS == 128 ? (a.rows + 3) / 4 : a.rows, room = uint32_t(sms * per_sm);
+    kernel<<<need < room ? need : room, block, 0, st>>>(a);
+    return cudaGetLastError();
+}
+template <int VEC, int PER, int MAX_THREADS>
+cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
     const uint32_t threads = ((a.width + VEC * PER - 1) / (VEC * PER) + 31) & ~31u;
-    if (threads == 32) block_norm_kernel<VEC, PER, false><<<(a.rows + 3) / 4, 128, 0, st>>>(a);
-    else block_norm_kernel<VEC, PER, true><<<a.rows, threads, 0, st>>>(a);
+    if (threads == 32) {
+        if (a.y_f32) return a.h_f32 ? launch_norm_kernel<VEC, PER, 128, true, true>(a, threads, st) : launch_norm_kernel<VEC, PER, 128, true, false>(a, threads, st);
+        return a.h_f32 ? launch_norm_kernel<VEC, PER, 128, false, true>(a, threads, st) : launch_norm_kernel<VEC, PER, 128, false, false>(a, threads, st);
+    }
+    if (a.y_f32) return a.h_f32 ? launch_norm_kernel<VEC, PER, MAX_THREADS, true, true>(a, threads, st) : launch_norm_kernel<VEC, PER, MAX_THREADS, true, false>(a, threads, st);
+    return a.h_f32 ? launch_norm_kernel<VEC, PER, MAX_THREADS, false, true>(a, threads, st) : launch_norm_kernel<VEC, PER, MAX_THREADS, false, false>(a, threads, st);
 }
 
 }  // namespace
@@ -233,7 +254,8 @@ int m26b_block_norm_dev(const m26b_block_norm_args* args, void* stream, char* er
     a.y_pitch = y_pitch; a.h_pitch = h_pitch; a.n_pitch = n_pitch;
     a.post_w = in.post_w; a.gate = in.gate; a.residual = in.residual; a.pre_w = in.pre_w;
     a.gate_kind = gate_kind;
-    a.y_scale = in.y_scale; a.residual_scale = in.residual_scale; a.eps = in.eps;
+    a.y_scale = n_planes ? in.y_scale : 0.0f; a.residual_scale = in.residual ? in.residual_scale : 0.0f; a.eps = in.eps;
+    a.inv_width = 1.0f / float(width);
     a.rows = rows; a.width = width; a.h_out = in.h_out; a.n_out = in.n_out;
     see(in.post_w, w_dtype); see(in.pre_w, w_dtype); see(in.residual, h_dtype); see(in.h_out, h_dtype); see(in.n_out, n_dtype);
     if (gate_kind == kGateToken) elem |= reinterpret_cast<uintptr_t>(in.gate) & 3;
@@ -241,16 +263,17 @@ int m26b_block_norm_dev(const m26b_block_norm_args* args, void* stream, char* er
     if (elem) { set_msg(err, errlen, "m26b block norm: a pointer is not aligned to its element size"); return 1; }
     if (!rows) return 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e;
     if (!vec && (width | (n_planes ? y_pitch : 0) | (in.residual || in.h_out ? h_pitch : 0) | (in.n_out ? n_pitch : 0)) % 8 == 0) {
-        if (width <= 8192) launch_norm<8, 1>(a, st);
-        else if (width <= 16384) launch_norm<8, 2>(a, st);
-        else launch_norm<8, 4>(a, st);
+        if (width <= 2048) e = launch_norm<8, 1, 256>(a, st);
+        else if (width <= 8192) e = launch_norm<8, 2, 512>(a, st);
+        else if (width <= 16384) e = launch_norm<8, 2, 1024>(a, st);
+        else e = launch_norm<8, 4, 1024>(a, st);
     } else {
-        if (width <= 4096) launch_norm<1, 4>(a, st);
-        else if (width <= 16384) launch_norm<1, 16>(a, st);
-        else launch_norm<1, 32>(a, st);
+        if (width <= 8192) e = launch_norm<1, 8, 1024>(a, st);
+        else if (width <= 16384) e = launch_norm<1, 16, 1024>(a, st);
+        else e = launch_norm<1, 32, 1024>(a, st);
     }
-    const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) { set_err(err, errlen, "m26b block norm launch", e); return 2; }
     return 0;
 }
