@@ -14,6 +14,8 @@
 #include <cuda_runtime.h>
 #include <cstdint>
 
+#include "sm100_ptx.cuh"
+
 namespace m26b {
 
 enum { kGateNone = 0, kGateToken = 1, kGateChannel = 2, kGateElement = 3 };
@@ -162,6 +164,8 @@ __global__ void __launch_bounds__(MAX_THREADS) block_norm_kernel(const NormArgs 
     };
 #pragma unroll
     for (int j = 0; j < PER; ++j) { ry[j].zero(); rh[j].zero(); rg[j].zero(); }
+    grid_dep_wait();                                 // the block's output comes from the stream's earlier kernels
+    grid_dep_launch();
     if (row < p.rows) request(row);
     for (uint32_t turn = 0; row < p.rows; row += rows_at_once, ++turn) {
         float (*slots)[32] = slots_all[turn & 1];    // the other set may still be read by slower warps of the row before

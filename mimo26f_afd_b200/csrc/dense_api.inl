@@ -15,6 +15,7 @@ namespace {
 
 constexpr uint32_t kLinearMaxDim = 1u << 20;
 constexpr uint32_t kLinearPassRows = 8192;      // tokens per pass: bounds the workspace at 2 x 8192 x k bytes
+constexpr uint32_t kLinearDirectRows = 32;      // requests up to this many tokens take aligned activations as they are
 
 // The gated weight image [rows][k_pad] seen as [blocks of 128 rows][128][k_pad] (blocks alternate gate / up), boxes of 128 elements x
 // 64 rows x 2 blocks: one copy brings 64 gate rows and the 64 up rows of the same features.
@@ -73,10 +74,10 @@ int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool 
 
 uint32_t linear_rows_cap(uint32_t rows) { return ((rows < kLinearPassRows ? rows : kLinearPassRows) + 15) & ~15u; }
 
-template <int B_ROWS, int PIECES, bool GATED>
+template <int B_ROWS, int PIECES, bool GATED, bool DIRECT>
 cudaError_t launch_linear(const m26b_linear* L, const TokenMaps& mx, const LinearArgs& a, cudaStream_t st) {
     using T = LinearTile<B_ROWS, PIECES>;
-    const auto kernel = linear_w4_kernel<B_ROWS, PIECES, GATED>;
+    const auto kernel = linear_w4_kernel<B_ROWS, PIECES, GATED, DIRECT>;
     const int smem = int(sizeof(LinearSmem<B_ROWS, PIECES>)) + 1024;
     static std::atomic<uint64_t> opted{0};                             // one flag bit per device of this process
     const uint64_t bit = 1ull << (L->device & 63);
@@ -85,51 +86,51 @@ cudaError_t launch_linear(const m26b_linear* L, const TokenMaps& mx, const Linea
         if (e != cudaSuccess) return e;
         opted.fetch_or(bit, std::memory_order_relaxed);
     }
-    const uint32_t tiles = GATED ? (a.n + 63) / 64 : (a.n + kTileM - 1) / kTileM, tok_tiles = (a.rows + B_ROWS - 1) / B_ROWS;
+    const uint32_t feats = GATED ? 64 : kTileM, tiles = (a.n + feats - 1) / feats, tok_tiles = (a.rows + B_ROWS - 1) / B_ROWS;
     // K is split over a cluster while the CTAs still fit the SMs at once and each keeps at least two chunks
-    uint32_t split = 1;
-    while (split < 8 && uint64_t(tiles) * tok_tiles * split * 2 <= uint64_t(L->sms) * T::kCtasPerSm && a.chunks >= split * 4) split *= 2;
+    uint32_t log_split = 0;
+    while (log_split < 3 && (uint64_t(tiles) * tok_tiles << (log_split + 1)) <= uint64_t(L->sms) * T::kCtasPerSm && a.chunks >= 4u << log_split) ++log_split;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(tiles * split, tok_tiles); cfg.blockDim = dim3(kLinearThreads); cfg.dynamicSmemBytes = size_t(smem); cfg.stream = st;
+    cfg.gridDim = dim3(tiles << log_split, tok_tiles); cfg.blockDim = dim3(kLinearThreads); cfg.dynamicSmemBytes = size_t(smem); cfg.stream = st;
     cudaLaunchAttribute at[2]{};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = split; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    at[1].val.clusterDim.x = 1u << log_split; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, L->map_w, mx, a, split);
+    return cudaLaunchKernelEx(&cfg, kernel, L->map_w, mx, a, log_split);
 }
-template <int B_ROWS>
+template <int B_ROWS, bool DIRECT>
 cudaError_t launch_linear_tile(const m26b_linear* L, bool bf16, const TokenMaps& mx, const LinearArgs& a, cudaStream_t st) {
-    if (L->gated) return bf16 ? launch_linear<B_ROWS, 2, true>(L, mx, a, st) : launch_linear<B_ROWS, 1, true>(L, mx, a, st);
-    return bf16 ? launch_linear<B_ROWS, 2, false>(L, mx, a, st) : launch_linear<B_ROWS, 1, false>(L, mx, a, st);
+    if (L->gated) return bf16 ? launch_linear<B_ROWS, 2, true, DIRECT>(L, mx, a, st) : launch_linear<B_ROWS, 1, true, DIRECT>(L, mx, a, st);
+    return bf16 ? launch_linear<B_ROWS, 2, false, DIRECT>(L, mx, a, st) : launch_linear<B_ROWS, 1, false, DIRECT>(L, mx, a, st);
 }
 
 // One pass of at most kLinearPassRows tokens.
 int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x_scales, uint64_t x_pitch, uint32_t rows, void* y, int y_f32,
                 uint64_t y_pitch, uint8_t* ws, uint32_t* fault, cudaStream_t st, char* err, size_t errlen) {
     const uint32_t pieces = bf16 ? 2 : 1, rows_cap = linear_rows_cap(rows);
-    uint8_t* sf = ws + uint64_t(pieces) * rows_cap * L->k_pad;
-    SplitArgs sp{x, x_scales, x_pitch, 0, rows, L->k, L->k_pad, rows_cap, ws, sf};
     const uintptr_t xa = reinterpret_cast<uintptr_t>(x);
-    sp.vec = bf16 ? (xa % 16 == 0 && x_pitch % 8 == 0) : (xa % 8 == 0 && x_pitch % 8 == 0);
-    const uint64_t threads = uint64_t(rows) * (L->k_pad / 8);
-    const unsigned blocks = unsigned((threads + 255) / 256);
-    if (bf16) linear_split_kernel<2><<<blocks, 256, 0, st>>>(sp);
-    else linear_split_kernel<1><<<blocks, 256, 0, st>>>(sp);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) { set_err(err, errlen, "m26b linear stage launch", e); return 2; }
+    const int vec = bf16 ? (xa % 16 == 0 && x_pitch % 8 == 0) : (xa % 8 == 0 && x_pitch % 8 == 0);
+    uint8_t* sf = ws + uint64_t(pieces) * rows_cap * L->k_pad;
+    const LinearArgs a{L->sf, sf, rows, rows_cap, L->n, L->k_pad / kChunkK, y, y_f32, y_pitch, fault, x, x_scales, x_pitch, L->k};
     TokenMaps mx{};
-    for (int i = 0; i < 4; ++i)                     // the boxes a token tile of this request can use
-        if ((128u >> i) <= rows_cap && !make_map(&mx.box[i], false, ws, L->k_pad, uint64_t(pieces) * rows_cap, L->k_pad, 128u >> i)) {
-            set_msg(err, errlen, "m26b linear: cuTensorMapEncodeTiled failed for the activations");
-            return 2;
-        }
-    const LinearArgs a{L->sf, sf, rows, rows_cap, L->n, L->k_pad / kChunkK, y, y_f32, y_pitch, fault};
-    if (rows <= 16) e = launch_linear_tile<16>(L, bf16, mx, a, st);
-    else if (rows <= 32) e = launch_linear_tile<32>(L, bf16, mx, a, st);
-    else if (rows <= 64) e = launch_linear_tile<64>(L, bf16, mx, a, st);
-    else e = launch_linear_tile<128>(L, bf16, mx, a, st);
+    cudaError_t e;
+    if (rows <= kLinearDirectRows && vec) {
+        e = rows <= 16 ? launch_linear_tile<16, true>(L, bf16, mx, a, st) : launch_linear_tile<32, true>(L, bf16, mx, a, st);
+    } else {
+        const SplitArgs sp{x, x_scales, x_pitch, vec, rows, L->k, L->k_pad, rows_cap, rows <= 64 ? 64u : 128u, ws, sf};
+        const uint64_t threads = uint64_t(rows) * (L->k_pad / 8);
+        const unsigned blocks = unsigned((threads + 255) / 256);
+        e = bf16 ? launch_dependent(linear_split_kernel<2>, blocks, 256, 0, st, sp) : launch_dependent(linear_split_kernel<1>, blocks, 256, 0, st, sp);
+        if (e != cudaSuccess) { cudaGetLastError(); set_err(err, errlen, "m26b linear stage launch", e); return 2; }
+        for (int i = 0; i < 4; ++i)                     // the boxes a token tile of this request can use
+            if ((128u >> i) <= rows_cap && !make_map(&mx.box[i], false, ws, L->k_pad, uint64_t(pieces) * rows_cap, L->k_pad, 128u >> i)) {
+                set_msg(err, errlen, "m26b linear: cuTensorMapEncodeTiled failed for the activations");
+                return 2;
+            }
+        e = rows <= 64 ? launch_linear_tile<64, false>(L, bf16, mx, a, st) : launch_linear_tile<128, false>(L, bf16, mx, a, st);
+    }
     if (e != cudaSuccess) { cudaGetLastError(); set_err(err, errlen, "m26b linear launch", e); return 2; }
     return 0;
 }
@@ -148,8 +149,7 @@ cudaError_t launch_norm_kernel(const NormArgs& a, uint32_t threads, cudaStream_t
         resident[block / 32].store(per_sm, std::memory_order_relaxed);
     }
     const uint32_t need = MAX_THREADS == 128 ? (a.rows + 3) / 4 : a.rows, room = uint32_t(sms * per_sm);
-    kernel<<<need < room ? need : room, block, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch_dependent(kernel, need < room ? need : room, block, 0, st, a);
 }
 template <int VEC, int PER, int MAX_THREADS>
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
@@ -274,7 +274,7 @@ int m26b_block_norm_dev(const m26b_block_norm_args* args, void* stream, char* er
         else if (width <= 16384) e = launch_norm<1, 16, 1024>(a, st);
         else e = launch_norm<1, 32, 1024>(a, st);
     }
-    if (e != cudaSuccess) { set_err(err, errlen, "m26b block norm launch", e); return 2; }
+    if (e != cudaSuccess) { cudaGetLastError(); set_err(err, errlen, "m26b block norm launch", e); return 2; }
     return 0;
 }
 

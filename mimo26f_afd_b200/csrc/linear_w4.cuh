@@ -71,35 +71,43 @@ __global__ void __launch_bounds__(256) linear_prep_scales_kernel(LinearSrc src, 
 // ---- activations -> E4M3 pieces ------------------------------------------------------------------------------------
 // Scale byte of the leading piece for a block maximum (bits of a finite FP32 magnitude); the second piece's byte is 4 less.
 __device__ __forceinline__ uint32_t split_scale_byte(uint32_t amax_bits) {
-    if (!amax_bits) return 127u;
-    uint32_t sig; int exp;
-    split_f32(amax_bits, sig, exp);
-    const int s = exp - ((sig & 0x7fffffu) <= 0x600000u ? 8 : 7) + 127;
+    // exponent field - 8, one more when the significand is above 1.75 (448 = 1.75 * 2^8); zero and subnormal blocks end at the floor
+    const int s = int((amax_bits + 0x1fffffu) >> 23) - 8;
     return uint32_t(s < 4 ? 4 : s);                                            // at most 247
 }
-__device__ __forceinline__ uint32_t e4m3x2_rn(float lo, float hi) {
+__device__ __forceinline__ uint32_t e4m3x2_rn(uint32_t f16x2) {
     uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(f16x2));
     return r;
 }
-__device__ __forceinline__ float2 e4m3x2_f32(uint32_t pair) {
+__device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint32_t pair) {
     uint32_t h;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(pair)));
-    float lo, hi;
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(lo), "=f"(hi) : "r"(h));
-    return make_float2(lo, hi);
+    return h;
 }
-// Eight BF16 values (bits in the upper half of FP32 words) with the block's scale byte -> eight codes of each piece.
-__device__ __forceinline__ void split8(const float (&v)[8], uint32_t scale, bool bad, uint2& hi, uint2& lo) {
-    if (bad) { hi = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu); lo = make_uint2(0, 0); return; }
-    const float inv = __uint_as_float((254u - scale) << 23);                   // 2^(127 - scale), scale in 4..247
+// Largest magnitude of a K32 block, as FP32 bits: each of the block's four neighbouring lanes holds eight BF16 (`lanes`: those four
+// or more). Infinities and NaN order above every number.
+__device__ __forceinline__ uint32_t block_amax(const uint32_t (&w)[4], uint32_t lanes) {
+    uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    m = __vmaxu2(m, __shfl_xor_sync(lanes, m, 1));
+    m = __vmaxu2(m, __shfl_xor_sync(lanes, m, 2));
+    return max(m << 16, m & 0xffff0000u);
+}
+// Eight BF16 (pairs as in memory) under the block's scale byte -> eight codes of each piece. The scaled values, at most 448 with
+// eight significant bits, are exact in FP16 down to 2^-17 and off by 2^-25 at most below, far under the second piece's 2^-13
+// grid; their difference to the first piece is exact there too.
+__device__ __forceinline__ void split8(const uint32_t (&w)[4], uint32_t scale, bool bad, uint2& hi, uint2& lo) {
+    // 2^(127 - scale), scale in 4..247; a bad block is scaled by NaN and becomes NaN codes
+    const float inv = bad ? __int_as_float(0x7fc00000) : __uint_as_float((254u - scale) << 23);
     uint32_t h[4], l[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float a = v[2 * j] * inv, b = v[2 * j + 1] * inv;
-        h[j] = e4m3x2_rn(a, b);
-        const float2 d = e4m3x2_f32(h[j]);
-        l[j] = e4m3x2_rn((a - d.x) * 16.0f, (b - d.y) * 16.0f);
+        uint32_t a, r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(a) : "f"(__uint_as_float(w[j] & 0xffff0000u) * inv), "f"(__uint_as_float(w[j] << 16) * inv));
+        h[j] = e4m3x2_rn(a);
+        asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(f16x2_of_e4m3x2(h[j])));
+        asm("mul.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0x4c004c00u));         // 16
+        l[j] = e4m3x2_rn(r);
     }
     hi = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
     lo = make_uint2(l[0] | l[1] << 16, l[2] | l[3] << 16);
@@ -111,12 +119,14 @@ struct SplitArgs {
     uint64_t pitch;              // elements
     int vec;                     // rows start on 16-byte (BF16) / 8-byte (E4M3) boundaries
     uint32_t rows, k, k_pad, rows_cap;
+    uint32_t lo_row;             // scale-block row of the second piece's first token: 64 (one block per chunk) or 128 (two)
     uint8_t* q;                  // [PIECES][rows_cap][k_pad]
-    uint8_t* sf;                 // [128-token tile][chunk][PIECES][512]
+    uint8_t* sf;                 // [128-token tile][chunk][blocks][512]
 };
 // Four threads per K32 block, eight elements each.
 template <int PIECES>
 __global__ void __launch_bounds__(256) linear_split_kernel(const SplitArgs p) {
+    grid_dep_wait();             // x, and the workspace that an earlier call may still read
     grid_dep_launch();
     const uint32_t groups = p.k_pad / 8;
     const uint64_t id = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -128,26 +138,21 @@ __global__ void __launch_bounds__(256) linear_split_kernel(const SplitArgs p) {
     uint32_t scale = 127;
     uint2 hi = make_uint2(0, 0), lo = make_uint2(0, 0);
     if constexpr (PIECES == 2) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+        uint32_t w[4] = {0, 0, 0, 0};
         if (real) {
+            const uint16_t* x = static_cast<const uint16_t*>(p.x) + at;
             if (p.vec) {
-                load_elems<8>(p.x, 0, at, v);
+                const uint4 a = *reinterpret_cast<const uint4*>(x);
+                w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(uint32_t(static_cast<const uint16_t*>(p.x)[at + e]) << 16);
+                for (int e = 0; e < 4; ++e) w[e] = uint32_t(x[2 * e]) | uint32_t(x[2 * e + 1]) << 16;
             }
         }
-        uint32_t amax = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(v[e]) & 0x7fffffffu);
-        const uint32_t quad = 0xfu << (threadIdx.x & 28u);
-        amax = max(amax, __shfl_xor_sync(quad, amax, 1));
-        amax = max(amax, __shfl_xor_sync(quad, amax, 2));
+        const uint32_t amax = block_amax(w, 0xfu << (threadIdx.x & 28u));
         const bool bad = amax >= 0x7f800000u;
         if (!bad) scale = split_scale_byte(amax);
-        split8(v, scale, bad, hi, lo);
+        split8(w, scale, bad, hi, lo);
     } else if (real) {
         const uint8_t* x = static_cast<const uint8_t*>(p.x) + at;
         if (p.vec) {
@@ -165,9 +170,13 @@ __global__ void __launch_bounds__(256) linear_split_kernel(const SplitArgs p) {
     *reinterpret_cast<uint2*>(q) = hi;
     if constexpr (PIECES == 2) *reinterpret_cast<uint2*>(q + uint64_t(p.rows_cap) * p.k_pad) = lo;
     if ((g & 3u) == 0) {
-        uint8_t* sf = p.sf + (uint64_t(row >> 7) * (p.k_pad / kChunkK) + (kb >> 2)) * PIECES * kScaleBlockBytes + scale_block_offset(int(row & 127u), int(kb & 3u));
-        sf[0] = uint8_t(scale);
-        if constexpr (PIECES == 2) sf[kScaleBlockBytes] = uint8_t(scale - 4u);
+        const uint32_t blocks = PIECES == 2 && p.lo_row == 128 ? 2 : 1, r = row & 127u;
+        uint8_t* sf = p.sf + (uint64_t(row >> 7) * (p.k_pad / kChunkK) + (kb >> 2)) * blocks * kScaleBlockBytes;
+        sf[scale_block_offset(int(r), int(kb & 3u))] = uint8_t(scale);
+        if constexpr (PIECES == 2) {
+            const uint32_t lr = p.lo_row + r;
+            sf[(lr >> 7) * kScaleBlockBytes + scale_block_offset(int(lr & 127u), int(kb & 3u))] = uint8_t(scale - 4u);
+        }
     }
 }
 
@@ -182,6 +191,11 @@ struct LinearArgs {
     int y_f32;
     uint64_t y_pitch;            // elements
     uint32_t* fault;
+    // activations as the caller has them (DIRECT kernels): rows start on 16-byte (BF16) / 8-byte (E4M3) boundaries
+    const void* x;
+    const uint8_t* x_scales;
+    uint64_t x_pitch;
+    uint32_t k;
 };
 
 __device__ __forceinline__ float silu_gate(float g, float u) {
@@ -199,69 +213,167 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+// The pieces of a token tile are one MMA operand of PIECES * B_ROWS rows - the second piece's B_ROWS rows behind the first's - with
+// accumulator columns of their own, added in the epilogue: a narrow MMA costs what reading its 128 weight rows costs, so one
+// MMA twice as wide is cheaper than two (16 tokens, 16,384 x 4,096 gated: 660 cycles of issue per chunk with two).
 template <int B_ROWS, int PIECES>
 struct LinearTile {
-    static constexpr int kStageBytes = kTileM * 128 + PIECES * B_ROWS * 128 + (1 + PIECES) * kScaleBlockBytes;
+    static constexpr int kN = PIECES * B_ROWS, kSfb = kN > 128 ? 2 : 1;    // operand rows, scale blocks of a chunk
     static constexpr int kCtasPerSm = B_ROWS <= 32 ? 2 : 1;
-    static constexpr int kRedBytes = B_ROWS * kTileM * 4;          // partial sums of a split K, and the gate / up exchange
-    static constexpr int kBudget = (kCtasPerSm == 2 ? 113 : 226) * 1024 - 2048;
-    static constexpr int kFit = (kBudget - kRedBytes) / kStageBytes;
+    static constexpr int kStageBytes = kTileM * 128 + kN * 128 + (1 + kSfb) * kScaleBlockBytes;
+    static constexpr int kRedBytes = B_ROWS * kTileM * 4;                  // partial sums of a split K, and the gate / up exchange
+    static constexpr int kFit = ((kCtasPerSm == 2 ? 111 : 224) * 1024 - kRedBytes) / kStageBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
-    static constexpr uint32_t kCols = B_ROWS + 32 <= 64 ? 64 : B_ROWS + 32 <= 128 ? 128 : 256;
+    static constexpr uint32_t kCols = kN + 32 <= 64 ? 64 : kN + 32 <= 128 ? 128 : kN + 32 <= 256 ? 256 : 512;   // two scale slots of 16 columns
     static_assert(kStages >= 3, "too few stages");
 };
 template <int B_ROWS, int PIECES>
 struct LinearSmem {
     using T = LinearTile<B_ROWS, PIECES>;
     alignas(1024) uint8_t a[T::kStages][kTileM * 128];
-    alignas(1024) uint8_t b[T::kStages][PIECES * B_ROWS * 128];
+    alignas(1024) uint8_t b[T::kStages][T::kN * 128];
     alignas(128) uint8_t sfa[T::kStages][kScaleBlockBytes];
-    alignas(128) uint8_t sfb[T::kStages][PIECES * kScaleBlockBytes];
+    alignas(128) uint8_t sfb[T::kStages][T::kSfb * kScaleBlockBytes];
     alignas(16) float red[T::kRedBytes / 4];
     uint64_t full[T::kStages], empty[T::kStages], acc_full;
     uint32_t tmem_base, abort_flag;
 };
-constexpr int kLinearThreads = 192;              // producer warp, MMA warp, four epilogue warps
+constexpr int kConvWarps = 8;                    // epilogue warps: two per tensor-memory lane quadrant; the converters of DIRECT kernels
+constexpr int kLinearThreads = 64 + 32 * kConvWarps;     // a producer warp and an MMA warp in front
 
-// One CTA: one 128-row weight tile (blockIdx.x / split) x one token tile (blockIdx.y), over its share of the K chunks. The
-// `split` CTAs of a cluster share a tile; they add their partial sums over distributed shared memory in rank order, CTA r
-// finishing 1 / split of the tile's features, so the result does not depend on timing. Token tiles start on multiples of 128
+// Eight activations of one row as they lie in memory, and their block's scale byte if they have one. The address is valid
+// whatever the place (rows and columns beyond the request read its last row and first columns and are dropped when the values
+// are used): with no branch around them, the loads of a whole chunk stay in flight.
+template <int PIECES>
+struct RawX {
+    uint32_t w[PIECES == 2 ? 4 : 2];
+    uint32_t scale;
+    __device__ __forceinline__ void load(const LinearArgs& p, uint32_t row, uint32_t col) {
+        row = row < p.rows ? row : p.rows - 1;
+        col = col < p.k ? col : col & (kBlockK - 1);
+        const uint64_t at = uint64_t(row) * p.x_pitch + col;
+        if constexpr (PIECES == 2) {
+            const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + at);
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+            scale = 0;
+        } else {
+            const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.x) + at);
+            w[0] = a.x; w[1] = a.y;
+            scale = p.x_scales[uint64_t(row) * (p.k / kBlockK) + col / kBlockK];
+        }
+    }
+};
+
+// A converter warp of a DIRECT kernel: eight rows of chunks i, i + kLanes, ... of the request into their stages' token buffers,
+// sixteen lanes per row, two rows at a time. What a chunk costs is latency - the loads, then a chain of some twenty dependent
+// conversions and shuffles - so the warps work on different chunks and rows, and a warp takes its eight rows without a branch
+// (rows beyond the request repeat its last one into the tile's padding). Measured per chunk: 1,160 cycles for eight rows, 2,200
+// for sixteen, 3,570 for sixteen with the rows one pair after the other.
+template <int B_ROWS, int PIECES>
+struct LinearConverter {
+    static constexpr uint32_t kStages = LinearTile<B_ROWS, PIECES>::kStages, kParts = B_ROWS / 8;       // kParts warps share a chunk
+    // No more chunks at work than there are stages: a warp that has finished chunk i knows chunks up to i - kStages to be consumed,
+    // so with a step of at most kStages the parity it waits for next cannot be that of a stage's use before last.
+    static constexpr uint32_t kLanes = kConvWarps / kParts < kStages ? kConvWarps / kParts : kStages;
+    uint32_t row0, first, g, r0, c0, n_chunks;
+    RawX<PIECES> raw[4];
+
+    __device__ __forceinline__ LinearConverter(uint32_t cw, uint32_t lane, uint32_t c_first, uint32_t chunks)
+        : row0(cw % kParts * 8), first(cw / kParts), g(lane & 15u), r0(row0 + (lane >> 4)), c0(c_first), n_chunks(chunks) {}
+    __device__ __forceinline__ void request(const LinearArgs& p, uint32_t i) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) raw[v].load(p, r0 + 2 * v, (c0 + i) * kChunkK + g * 8);
+    }
+    template <class Smem>
+    __device__ __forceinline__ void run(const LinearArgs& p, Smem& s, uint32_t lane) {
+        if (row0 >= p.rows || first >= kLanes || first >= n_chunks) return;
+        request(p, first);
+        for (uint32_t i = first; i < n_chunks; i += kLanes) {
+            const uint32_t stage = i % kStages, phase = (i / kStages) & 1u;
+            const bool inside = (c0 + i) * kChunkK + g * 8 < p.k;
+            if (!__all_sync(0xffffffffu, mbar_wait(&s.empty[stage], phase ^ 1u, &s.abort_flag))) return;
+            uint32_t scale[4];
+            uint2 hi[4], lo[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const RawX<PIECES>& x = raw[v];
+                if constexpr (PIECES == 2) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = inside ? x.w[e] : 0u;
+                    const uint32_t amax = block_amax(w, 0xffffffffu);
+                    const bool bad = amax >= 0x7f800000u;
+                    scale[v] = bad ? 127u : split_scale_byte(amax);
+                    split8(w, scale[v], bad, hi[v], lo[v]);
+                } else {
+                    const bool nan = inside && x.scale == 255u;
+                    scale[v] = nan || !inside ? 127u : x.scale;
+                    hi[v] = nan ? make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu) : inside ? make_uint2(x.w[0], x.w[1]) : make_uint2(0, 0);
+                }
+            }
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const uint32_t r = r0 + 2 * v;
+                // 128-byte swizzle: 16-byte unit u of row r sits at unit u ^ (r % 8)
+                uint8_t* at = s.b[stage] + r * 128 + (((g >> 1) ^ (r & 7u)) << 4) + ((g & 1u) << 3);
+                *reinterpret_cast<uint2*>(at) = hi[v];
+                if constexpr (PIECES == 2) *reinterpret_cast<uint2*>(at + B_ROWS * 128) = lo[v];
+                if ((g & 3u) == 0) {
+                    s.sfb[stage][scale_block_offset(int(r), int(g >> 2))] = uint8_t(scale[v]);
+                    if constexpr (PIECES == 2) s.sfb[stage][scale_block_offset(int(B_ROWS + r), int(g >> 2))] = uint8_t(scale[v] - 4u);
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.full[stage]);
+            if (i + kLanes < n_chunks) request(p, i + kLanes);
+        }
+    }
+};
+
+// One CTA: one 128-row weight tile (blockIdx.x >> log_split) x one token tile (blockIdx.y), over its share of the K chunks. The
+// 1 << log_split CTAs of a cluster share a tile; they add their partial sums over distributed shared memory in rank order, each
+// finishing an equal part of the tile's features, so the result does not depend on timing. Token tiles start on multiples of 128
 // (their scale blocks hold 128 tokens): smaller B_ROWS serve requests of at most B_ROWS tokens.
-template <int B_ROWS, int PIECES, bool GATED>
+//
+// DIRECT (a few tokens): the epilogue warps, idle while the weights stream, turn the activations of each chunk into the
+// pieces in shared memory themselves; no second launch, no workspace. Every weight tile repeats that work, so larger requests
+// stage the pieces once (linear_split_kernel) and fetch them with TMA.
+template <int B_ROWS, int PIECES, bool GATED, bool DIRECT>
 __global__ void __launch_bounds__(kLinearThreads, (LinearTile<B_ROWS, PIECES>::kCtasPerSm))
-linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps maps_x, const LinearArgs p, const uint32_t split) {
+linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps maps_x, const LinearArgs p, const uint32_t log_split) {
+    static_assert(!DIRECT || B_ROWS * PIECES <= 128, "one scale block per chunk");
     using T = LinearTile<B_ROWS, PIECES>;
     using Smem = LinearSmem<B_ROWS, PIECES>;
     extern __shared__ uint8_t smem_raw[];
     Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t split = 1u << log_split;
     const uint32_t rank = split > 1 ? cluster_ctarank() : 0;
-    const uint32_t tile = blockIdx.x / split;
-    const uint32_t c0 = p.chunks * rank / split, c1 = p.chunks * (rank + 1) / split;
+    const uint32_t tile = blockIdx.x >> log_split;
+    const uint32_t c0 = p.chunks * rank >> log_split, c1 = p.chunks * (rank + 1) >> log_split;
     const uint32_t tok0 = blockIdx.y * B_ROWS;
     const uint32_t n_valid = p.rows - tok0 < B_ROWS ? p.rows - tok0 : B_ROWS, n_mma = (n_valid + 15) & ~15u;
     volatile uint32_t* abort_flag = &s.abort_flag;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < T::kStages; ++i) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 1); }
+        const uint32_t filled = DIRECT ? 1 + (p.rows + 7) / 8 : 1;         // the producer, and the converters that share a chunk
+        for (int i = 0; i < T::kStages; ++i) { mbar_init(&s.full[i], filled); mbar_init(&s.empty[i], 1); }
         mbar_init(&s.acc_full, 1);
         s.abort_flag = 0;
         mbar_init_fence();
     }
-    if (warp == 1) { tmem_alloc(&s.tmem_base, T::kCols); tmem_relinquish(); }
-    tc_fence_before();
     __syncthreads();
-    tc_fence_after();
-    const uint32_t tb = s.tmem_base;
-    if (split > 1) cluster_arrive();         // "this CTA has started": its shared memory may be written from now on
+    if (split > 1) cluster_arrive();             // "this CTA has started": its shared memory may be written from now on
+    grid_dep_launch();
 
     if (warp == 0) {
         // ------------------------------------------------------------ producer
         if (elect_one()) {
             tma_prefetch_desc(&map_w);
             const uint32_t n_chunks = c1 - c0;
-            const uint32_t tx = kTileM * 64 + PIECES * n_mma * 128 + (1 + PIECES) * kScaleBlockBytes;
-            const uint8_t* sfb_g = p.sfb + uint64_t(tok0 >> 7) * p.chunks * PIECES * kScaleBlockBytes;
+            const uint32_t tx = kTileM * 64 + kScaleBlockBytes + (DIRECT ? 0 : PIECES * n_mma * 128 + T::kSfb * kScaleBlockBytes);
+            const uint8_t* sfb_g = p.sfb + uint64_t(tok0 >> 7) * p.chunks * T::kSfb * kScaleBlockBytes;
             auto weights = [&](uint32_t i, uint32_t st) {
                 const uint32_t c = c0 + i;
                 mbar_expect_tx(&s.full[st], tx);
@@ -273,31 +385,33 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                     bulk_load(s.sfa[st], p.sfa + ((uint64_t(tile >> 1) * p.chunks + c) * 2 + (tile & 1)) * kScaleBlockBytes, kScaleBlockBytes, &s.full[st]);
                 }
             };
-            // the weights do not depend on the kernel that stages the activations: their first stages are requested before it ends
+            // the weights depend on no earlier kernel: their first stages are requested before the stream's last one ends
             const uint32_t early = n_chunks < uint32_t(T::kStages) ? n_chunks : uint32_t(T::kStages);
             for (uint32_t i = 0; i < early; ++i) weights(i, i);
-            grid_dep_wait();
+            if constexpr (!DIRECT) grid_dep_wait();
             uint32_t stage = 0, phase = 0;
             for (uint32_t i = 0; i < n_chunks; ++i) {
                 if (i >= early) {
                     if (!mbar_wait(&s.empty[stage], phase ^ 1u, abort_flag)) { atomicOr(p.fault, uint32_t(kFaultPipeline)); break; }
                     weights(i, stage);
                 }
-                const uint32_t c = c0 + i;
+                if constexpr (!DIRECT) {
+                    const uint32_t c = c0 + i;
 #pragma unroll
-                for (int piece = 0; piece < PIECES; ++piece) {
-                    uint32_t r = 0;
+                    for (int piece = 0; piece < PIECES; ++piece) {
+                        uint32_t r = 0;
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const uint32_t box = 128u >> b;
-                        if (box <= B_ROWS && n_mma - r >= box) {
-                            tma_load_2d(s.b[stage] + (piece * B_ROWS + r) * 128, &maps_x.box[b], int(c * kChunkK),
-                                        int(piece * p.rows_cap + tok0 + r), &s.full[stage]);
-                            r += box;
+                        for (int b = 0; b < 4; ++b) {
+                            const uint32_t box = 128u >> b;
+                            if (box <= B_ROWS && n_mma - r >= box) {
+                                tma_load_2d(s.b[stage] + (piece * B_ROWS + r) * 128, &maps_x.box[b], int(c * kChunkK),
+                                            int(piece * p.rows_cap + tok0 + r), &s.full[stage]);
+                                r += box;
+                            }
                         }
                     }
+                    bulk_load(s.sfb[stage], sfb_g + uint64_t(c) * T::kSfb * kScaleBlockBytes, T::kSfb * kScaleBlockBytes, &s.full[stage]);
                 }
-                bulk_load(s.sfb[stage], sfb_g + uint64_t(c) * PIECES * kScaleBlockBytes, PIECES * kScaleBlockBytes, &s.full[stage]);
                 if (++stage == uint32_t(T::kStages)) { stage = 0; phase ^= 1u; }
             }
             if (*abort_flag) {                     // a wait ran out: leave no copy of this CTA in flight behind
@@ -311,25 +425,29 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         if (split > 1) cluster_wait();
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issue
+        tmem_alloc(&s.tmem_base, T::kCols);      // while the first loads are under way; the epilogue warps learn the address below
+        tmem_relinquish();
+        tc_fence_before();
+        named_bar_sync(1, 32 + 32 * kConvWarps);
+        tc_fence_after();
+        const uint32_t tb = s.tmem_base;
         if (elect_one()) {
-            const uint32_t idesc0 = idesc_mx(kFmtE2M1, kFmtE4M3, n_mma, 0, 0);
+            const uint32_t idesc0 = idesc_mx(kFmtE2M1, kFmtE4M3, (PIECES - 1) * B_ROWS + n_mma, 0, 0);
+            const uint64_t a_desc0 = desc_sw128(smem_u32(s.a[0])), b_desc0 = desc_sw128(smem_u32(s.b[0]));
+            const uint64_t sfa_desc0 = desc_scale_block(smem_u32(s.sfa[0])), sfb_desc0 = desc_scale_block(smem_u32(s.sfb[0]));
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (uint32_t c = c0; c < c1; ++c) {
                 if (!mbar_wait(&s.full[stage], phase, abort_flag)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t t_sf = tb + B_ROWS + (c & 1u) * 16u;      // consecutive chunks alternate between two scale slots
-                tc_cp_scales(t_sf, desc_scale_block(smem_u32(s.sfa[stage])));
+                const uint32_t t_sf = tb + T::kN + (c & 1u) * 16u;       // consecutive chunks alternate between two scale slots
+                tc_cp_scales(t_sf, sfa_desc0 + stage * (sizeof(s.sfa[0]) >> 4));
 #pragma unroll
-                for (int piece = 0; piece < PIECES; ++piece) tc_cp_scales(t_sf + 4 + 4 * piece, desc_scale_block(smem_u32(s.sfb[stage]) + piece * kScaleBlockBytes));
-                const uint64_t ad = desc_sw128(smem_u32(s.a[stage]));
+                for (int b = 0; b < T::kSfb; ++b) tc_cp_scales(t_sf + 4 + 4 * b, sfb_desc0 + stage * (sizeof(s.sfb[0]) >> 4) + b * (kScaleBlockBytes >> 4));
+                const uint64_t ad = a_desc0 + stage * (sizeof(s.a[0]) >> 4), bd = b_desc0 + stage * (sizeof(s.b[0]) >> 4);
 #pragma unroll
-                for (int piece = 0; piece < PIECES; ++piece) {
-                    const uint64_t bd = desc_sw128(smem_u32(s.b[stage]) + piece * B_ROWS * 128);
-#pragma unroll
-                    for (uint32_t kb = 0; kb < 4; ++kb)
-                        tc_mma_mx(tb, ad + 2 * kb, bd + 2 * kb, idesc0 | (kb << 4) | (kb << 29), t_sf, t_sf + 4 + 4 * piece, (c != c0 || piece || kb) ? 1u : 0u);
-                }
+                for (uint32_t kb = 0; kb < 4; ++kb)
+                    tc_mma_mx(tb, ad + 2 * kb, bd + 2 * kb, idesc0 | (kb << 4) | (kb << 29), t_sf, t_sf + 4, (c != c0 || kb) ? 1u : 0u);
                 tc_commit(&s.empty[stage]);
                 if (++stage == uint32_t(T::kStages)) { stage = 0; phase ^= 1u; }
             }
@@ -339,8 +457,16 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         __syncwarp();
         if (split > 1) cluster_wait();
     } else {
+        named_bar_sync(1, 32 + 32 * kConvWarps);
+        tc_fence_after();
+        const uint32_t tb = s.tmem_base;
+        if constexpr (DIRECT) {
+            LinearConverter<B_ROWS, PIECES> conv(uint32_t(warp - 2), uint32_t(lane), c0, c1 - c0);
+            grid_dep_wait();                     // the activations come from the stream's earlier kernels
+            conv.run(p, s, uint32_t(lane));
+        }
         // ------------------------------------------------------------ epilogue, first half: tensor memory -> where it is added
-        const uint32_t q = uint32_t(warp) & 3u;
+        const uint32_t q = uint32_t(warp) & 3u;            // lane quadrant; the quadrant's two warps take every other sixteen tokens
         const uint32_t row = q * 32u + lane;               // weight row of the tile
         const bool ok = mbar_wait(&s.acc_full, 0, abort_flag);
         __syncwarp();
@@ -349,20 +475,22 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             tc_fence_after();
             const uint32_t t_acc = tb + ((q * 32u) << 16);
             // owner of a row and its place there: features are dealt in equal runs, gate and up of a feature together
-            const uint32_t per = kTileM / split;
-            uint32_t owner, slot;
-            if constexpr (GATED) {
-                const uint32_t f = row & 63u, half = per / 2;
-                owner = f / half; slot = (row >> 6) * half + f % half;
-            } else {
-                owner = row / per; slot = row % per;
-            }
-            const uint32_t base = split > 1 ? cluster_map(smem_u32(s.red), owner) : smem_u32(s.red);
+            const uint32_t log_run = (GATED ? 6 : 7) - log_split, f = GATED ? row & 63u : row;
+            const uint32_t owner = f >> log_run, slot = (f & ((1u << log_run) - 1)) + (GATED ? (row >> 6) << log_run : 0);
+            const uint32_t base = (split > 1 ? cluster_map(smem_u32(s.red), owner) : smem_u32(s.red)) + slot * 4;
             const uint32_t feat = tile * kTileM + row;
-            for (uint32_t col = 0; col < n_mma; col += 16) {
+            for (uint32_t col = uint32_t(warp - 2) / 4 * 16; col < n_mma; col += 32) {
                 uint32_t r[16];
                 tmem_ld16(t_acc + col, r);
-                tmem_wait_ld();
+                if constexpr (PIECES == 2) {
+                    uint32_t l[16];
+                    tmem_ld16(t_acc + B_ROWS + col, l);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(l[j]));
+                } else {
+                    tmem_wait_ld();
+                }
                 if (!GATED && split == 1) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
@@ -370,30 +498,31 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
-                        st_cluster_f32(base + ((rank * n_mma + col + j) * per + slot) * 4, __uint_as_float(r[j]));
+                        if (col + j < n_valid) st_cluster_f32(base + (((rank * n_valid + col + j) << (7 - log_split)) << 2), __uint_as_float(r[j]));
                 }
             }
             tc_fence_before();
         }
     }
-    __syncthreads();
-    if (warp == 1) tmem_dealloc(tb, T::kCols);
-    if (!GATED && split == 1) return;
     if (split > 1) cluster_sync_all();
-    // ------------------------------------------------------------ epilogue, second half: partial sums in rank order
-    const uint32_t per = kTileM / split, feats = GATED ? per / 2 : per;
-    const uint32_t feat0 = GATED ? tile * 64 + rank * feats : tile * kTileM + rank * feats;
-    for (uint32_t i = threadIdx.x; i < n_valid * feats; i += kLinearThreads) {
-        const uint32_t col = i / feats, f = i % feats;
-        if (feat0 + f >= p.n) continue;
-        float v = 0.0f, u = 0.0f;
-        for (uint32_t r = 0; r < split; ++r) {
-            const float* from = s.red + (r * n_mma + col) * per + f;
-            v += from[0];
-            if constexpr (GATED) u += from[feats];
+    else __syncthreads();
+    if (GATED || split > 1) {
+        // -------------------------------------------------------- epilogue, second half: partial sums in rank order
+        const uint32_t log_feats = (GATED ? 6 : 7) - log_split, feats = 1u << log_feats;
+        const uint32_t feat0 = tile * (GATED ? 64 : kTileM) + rank * feats;
+        for (uint32_t i = threadIdx.x; i < n_valid << log_feats; i += kLinearThreads) {
+            const uint32_t f = i & (feats - 1), col = i >> log_feats;
+            if (feat0 + f >= p.n) continue;
+            const float* from = s.red + (col << (7 - log_split)) + f;
+            float v = 0.0f, u = 0.0f;
+            for (uint32_t r = 0; r < split; ++r, from += n_valid << (7 - log_split)) {
+                v += from[0];
+                if constexpr (GATED) u += from[feats];
+            }
+            store_y(p, tok0 + col, feat0 + f, GATED ? silu_gate(v, u) : v);
         }
-        store_y(p, tok0 + col, feat0 + f, GATED ? silu_gate(v, u) : v);
     }
+    if (warp == 1) tmem_dealloc(s.tmem_base, T::kCols);
 }
 
 }  // namespace m26b

@@ -117,6 +117,27 @@ def test_linear_extents(torch, n, k):
     check(torch, run(x, rows), y, rounded(y, bound, False))
 
 
+@pytest.mark.parametrize("rows", [1, 3, 8, 13, 16, 23, 32, 64, 128])
+@pytest.mark.parametrize("n", [9000, 30000])
+def test_many_weight_tiles_with_many_chunks_each(torch, rows, n):
+    """Enough tiles that K is hardly split: every stage of the pipeline is reused several times in one CTA."""
+    import mimo26f_afd_b200 as M
+
+    k = 4096
+    g = gen(torch, rows + n)
+    w, s = make_weights(torch, n, k, g)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(torch.bfloat16)
+    q = torch.randint(0, 127, (rows, k), dtype=torch.uint8, device="cuda", generator=g)
+    xs = torch.randint(110, 130, (rows, k // 32), dtype=torch.uint8, device="cuda", generator=g)
+    run = Runner(torch, M.Linear.new(w, s, n, k), rows)
+    W = weight_f64(torch, w, s)
+    y, bound = product_and_bound(torch, x.double(), W)
+    check(torch, run(x, rows), y, rounded(y, bound, False))
+    y, bound = product_and_bound(torch, e4m3_f64(torch, q, xs), W, quantised=True)
+    check(torch, run(q, rows, x_scales=xs), y, rounded(y, bound, False))
+    assert int(run.fault) == 0
+
+
 @pytest.mark.parametrize("rows", [1, 16, 40, 130])
 @pytest.mark.parametrize("n,k", [(64, 128), (65, 160), (320, 4096), (1, 32), (129, 96), (200, 1024)])
 def test_gated(torch, rows, n, k):
@@ -238,7 +259,7 @@ def test_scale_bytes_at_the_ends_of_their_range(torch):
         assert bool((off <= (rounded(y, bound, False) + 2.0**-126)[:, keep]).all())
 
 
-@pytest.mark.parametrize("rows", [3, 40, 150])
+@pytest.mark.parametrize("rows", [3, 20, 40, 150])
 @pytest.mark.parametrize("x_off,x_pad,y_off,y_pad", [(0, 8, 0, 5), (1, 3, 1, 0), (3, 0, 2, 7), (8, 16, 0, 64)])
 def test_pitches_and_alignment_and_what_lies_between_the_rows(torch, rows, x_off, x_pad, y_off, y_pad):
     import mimo26f_afd_b200 as M
@@ -344,16 +365,16 @@ def test_linear_refusals(torch):
     n, k = 64, 64
     w, s = make_weights(torch, n, k, gen(torch, 16))
     layer = M.Linear.new(w, s, n, k)
-    x = torch.zeros(4, k, dtype=torch.bfloat16, device="cuda")
-    y = torch.zeros(4, n, device="cuda")
-    ws = torch.empty(layer.workspace_bytes(4), dtype=torch.uint8, device="cuda")
+    x = torch.zeros(40, k, dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros(40, n, device="cuda")
+    ws = torch.empty(layer.workspace_bytes(40), dtype=torch.uint8, device="cuda")
     f = torch.zeros(1, dtype=torch.int32, device="cuda")
     ok = dict(y_dtype=1, workspace=ws, fault=f)
-    M.linear_dev(layer, x, 4, y, **ok)
+    M.linear_dev(layer, x, 40, y, **ok)
     M.linear_dev(layer, None, 0, None)                          # no rows: no work, nothing needed
     for rows, kw in ((4, dict(ok, x_dtype=1)), (4, dict(ok, x_dtype=3)), (4, dict(ok, y_dtype=2)), (4, dict(ok, x_dtype=2)), (4, dict(ok, x_pitch=k - 1)),
-                     (4, dict(ok, y_pitch=n - 1)), (4, dict(ok, fault=None)), (4, dict(ok, workspace=None)), (4, dict(ok, workspace=ws[:-1])),
-                     (4, dict(ok, workspace=ws[16:])), (17, ok), (4, dict(ok, workspace=ws.data_ptr()))):
+                     (4, dict(ok, y_pitch=n - 1)), (4, dict(ok, fault=None)), (40, dict(ok, workspace=None)), (40, dict(ok, workspace=ws[:-1])),
+                     (40, dict(ok, workspace=ws[16:])), (49, ok), (40, dict(ok, workspace=ws.data_ptr()))):
         with pytest.raises(M.ExpertError) as e:
             M.linear_dev(layer, x, rows, y, **kw)
         assert e.value.code == 1
@@ -362,7 +383,7 @@ def test_linear_refusals(torch):
             M.linear_dev(layer, xx, 4, yy, **ok)
         assert e.value.code == 1
     torch.cuda.synchronize()
-    assert layer.workspace_bytes(0) == 0 and layer.workspace_bytes(8192) == layer.workspace_bytes(1 << 20)
+    assert layer.workspace_bytes(0) == 0 < layer.workspace_bytes(1) and layer.workspace_bytes(8192) == layer.workspace_bytes(1 << 20)
 
 
 # --------------------------------------------------------------------------------------------------------------- norm
