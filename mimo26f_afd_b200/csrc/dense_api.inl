@@ -8,7 +8,8 @@ struct m26b_linear {
     uint32_t n = 0, k = 0, k_pad = 0;
     bool gated = false;
     int device = 0, sms = 0;
-    CUtensorMap map_w;
+    uint32_t tiles = 0;                         // 128-row tiles of the image (even)
+    CUtensorMap map_w, map_sf;
 };
 
 namespace {
@@ -16,19 +17,6 @@ namespace {
 constexpr uint32_t kLinearMaxDim = 1u << 20;
 constexpr uint32_t kLinearPassRows = 8192;      // tokens per pass: bounds the workspace at 2 x 8192 x k bytes
 constexpr uint32_t kLinearDirectRows = 32;      // requests up to this many tokens take aligned activations as they are
-
-// The gated weight image [rows][k_pad] seen as [blocks of 128 rows][128][k_pad] (blocks alternate gate / up), boxes of 128 elements x
-// 64 rows x 2 blocks: one copy brings 64 gate rows and the 64 up rows of the same features.
-bool make_map_gated(CUtensorMap* m, void* base, uint64_t k_pad, uint64_t rows) {
-    EncodeTiledFn f = encode_fn();
-    if (!f) return false;
-    cuuint64_t dims[3] = {k_pad, uint64_t(kTileM), rows / kTileM};
-    cuuint64_t strides[2] = {k_pad / 2, uint64_t(kTileM) * (k_pad / 2)};
-    cuuint32_t box[3] = {128, kTileM / 2, 2};
-    cuuint32_t es[3] = {1, 1, 1};
-    return f(m, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 3, base, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
 
 int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool gated, uint32_t n, uint32_t k, m26b_linear** out, char* err,
                size_t errlen) {
@@ -41,9 +29,10 @@ int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool 
     if (!L) { set_msg(err, errlen, "m26b linear: out of host memory"); return 2; }
     L->n = n; L->k = k; L->gated = gated;
     L->k_pad = (k + kChunkK - 1) / kChunkK * kChunkK;
-    const uint64_t feats = gated ? kTileM : kPairM;                    // output features per 256 image rows
-    const uint64_t rows = (n + feats - 1) / feats * kPairM, chunks = L->k_pad / kChunkK;
-    const uint64_t w_bytes = rows * (L->k_pad / 2), sf_bytes = rows / kTileM * chunks * kScaleBlockBytes;
+    const uint32_t feats = gated ? kTileM : kPairM;                    // output features of two tiles
+    L->tiles = (n + feats - 1) / feats * 2;
+    const uint64_t rows = uint64_t(L->tiles) * kTileM, chunks = L->k_pad / kChunkK;
+    const uint64_t w_bytes = rows * (L->k_pad / 2), sf_bytes = L->tiles * chunks * kScaleBlockBytes;
     auto fail = [&](const char* what, cudaError_t e) {
         set_err(err, errlen, what, e);
         m26b_linear_free(L);
@@ -63,7 +52,7 @@ int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool 
     linear_prep_scales_kernel<<<L->sms * 8, 256>>>(src, gated, n, k, uint32_t(chunks), sf_bytes, L->sf);
     if ((e = cudaGetLastError()) != cudaSuccess) return fail("m26b linear prepare launch", e);
     if ((e = cudaDeviceSynchronize()) != cudaSuccess) return fail("m26b linear prepare", e);
-    if (!(gated ? make_map_gated(&L->map_w, L->w, L->k_pad, rows) : make_map(&L->map_w, true, L->w, L->k_pad, rows, L->k_pad / 2, kTileM))) {
+    if (!make_map(&L->map_w, true, L->w, L->k_pad, rows, L->k_pad / 2, kTileM) || !make_sf_map(&L->map_sf, L->sf, L->tiles * chunks, 1)) {
         set_msg(err, errlen, "m26b linear: cuTensorMapEncodeTiled failed for the weights");
         m26b_linear_free(L);
         return 2;
@@ -106,6 +95,45 @@ cudaError_t launch_linear_tile(const m26b_linear* L, bool bf16, const TokenMaps&
     return bf16 ? launch_linear<B_ROWS, 2, false, DIRECT>(L, mx, a, st) : launch_linear<B_ROWS, 1, false, DIRECT>(L, mx, a, st);
 }
 
+// How many CTAs of the pair kernel the device holds at once (an even number, at most one per SM); 0 if it cannot place a pair.
+template <int PIECES, bool GATED>
+int linear_pair_ctas(const m26b_linear* L) {
+    static std::atomic<int> known[64]{};                               // by device of this process: CTAs + 1
+    std::atomic<int>& mine = known[L->device & 63];
+    int ctas = mine.load(std::memory_order_relaxed);
+    if (ctas) return ctas - 1;
+    const auto kernel = linear_pair_kernel<PIECES, GATED>;
+    const int smem = int(sizeof(LinearPairSmem<PIECES>)) + 1024;
+    int clusters = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(unsigned(L->sms & ~1)); cfg.blockDim = dim3(kLpThreads); cfg.dynamicSmemBytes = size_t(smem);
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = 2; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+        cfg.attrs = &at; cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) clusters = 0;
+    }
+    cudaGetLastError();
+    ctas = 2 * clusters < (L->sms & ~1) ? 2 * clusters : (L->sms & ~1);
+    mine.store(ctas + 1, std::memory_order_relaxed);
+    return ctas;
+}
+template <int PIECES, bool GATED>
+cudaError_t launch_linear_pair(const m26b_linear* L, const LinearPairMaps& maps, const LinearArgs& a, cudaStream_t st) {
+    const uint32_t m_pairs = L->tiles / 2, items = m_pairs * ((a.rows + kLpTokens - 1) / kLpTokens);
+    const uint32_t room = uint32_t(linear_pair_ctas<PIECES, GATED>(L));
+    return launch_dependent(linear_pair_kernel<PIECES, GATED>, 2 * items < room ? 2 * items : room, kLpThreads, sizeof(LinearPairSmem<PIECES>) + 1024, st,
+                            maps, a, m_pairs, items);
+}
+// Whether a request runs on CTA pairs: PAIR_RULE
+bool linear_on_pairs(const m26b_linear* L, bool bf16, uint32_t rows) {
+    const uint64_t items = uint64_t(L->tiles / 2) * ((rows + kLpTokens - 1) / kLpTokens);
+    if (rows <= 128 || items * 4 < uint64_t(L->sms)) return false;
+    const int ctas = L->gated ? (bf16 ? linear_pair_ctas<2, true>(L) : linear_pair_ctas<1, true>(L)) : (bf16 ? linear_pair_ctas<2, false>(L) : linear_pair_ctas<1, false>(L));
+    return ctas > 0;
+}
+
 // One pass of at most kLinearPassRows tokens.
 int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x_scales, uint64_t x_pitch, uint32_t rows, void* y, int y_f32,
                 uint64_t y_pitch, uint8_t* ws, uint32_t* fault, cudaStream_t st, char* err, size_t errlen) {
@@ -124,12 +152,26 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
         const unsigned blocks = unsigned((threads + 255) / 256);
         e = bf16 ? launch_dependent(linear_split_kernel<2>, blocks, 256, 0, st, sp) : launch_dependent(linear_split_kernel<1>, blocks, 256, 0, st, sp);
         if (e != cudaSuccess) { cudaGetLastError(); set_err(err, errlen, "m26b linear stage launch", e); return 2; }
-        for (int i = 0; i < 4; ++i)                     // the boxes a token tile of this request can use
-            if ((128u >> i) <= rows_cap && !make_map(&mx.box[i], false, ws, L->k_pad, uint64_t(pieces) * rows_cap, L->k_pad, 128u >> i)) {
-                set_msg(err, errlen, "m26b linear: cuTensorMapEncodeTiled failed for the activations");
-                return 2;
+        const uint64_t map_rows = uint64_t(pieces) * rows_cap;
+        const auto boxes = [&](CUtensorMap* to, int count) {            // the boxes a token tile of this request can use
+            for (int i = 0; i < count; ++i)
+                if ((128u >> i) <= rows_cap && !make_map(&to[i], false, ws, L->k_pad, map_rows, L->k_pad, 128u >> i)) return false;
+            return true;
+        };
+        bool maps_ok;
+        if (linear_on_pairs(L, bf16, rows)) {
+            LinearPairMaps pm{};
+            pm.w = L->map_w; pm.sfa = L->map_sf;
+            maps_ok = boxes(pm.tok, 5) && make_sf_map(&pm.sfb, sf, uint64_t((rows + 127) / 128) * a.chunks * pieces, pieces);
+            if (maps_ok) {
+                if (L->gated) e = bf16 ? launch_linear_pair<2, true>(L, pm, a, st) : launch_linear_pair<1, true>(L, pm, a, st);
+                else e = bf16 ? launch_linear_pair<2, false>(L, pm, a, st) : launch_linear_pair<1, false>(L, pm, a, st);
             }
-        e = rows <= 64 ? launch_linear_tile<64, false>(L, bf16, mx, a, st) : launch_linear_tile<128, false>(L, bf16, mx, a, st);
+        } else {
+            maps_ok = boxes(mx.box, 4);
+            if (maps_ok) e = rows <= 64 ? launch_linear_tile<64, false>(L, bf16, mx, a, st) : launch_linear_tile<128, false>(L, bf16, mx, a, st);
+        }
+        if (!maps_ok) { set_msg(err, errlen, "m26b linear: cuTensorMapEncodeTiled failed for the activations"); return 2; }
     }
     if (e != cudaSuccess) { cudaGetLastError(); set_err(err, errlen, "m26b linear launch", e); return 2; }
     return 0;

@@ -16,7 +16,6 @@
 // A K32 block with an infinity or a NaN becomes a block of NaN: every output of that row is NaN.
 //
 // Weights are the MMA "A" operand (M = 128 rows per tile), tokens the "B" operand (N = token tile), as in gemm_mx.cuh.
-// For the gated form a 128-row tile holds 64 gate rows and the 64 up rows of the same features.
 #pragma once
 #include "gemm_mx.cuh"
 #include "block_norm.cuh"
@@ -24,23 +23,35 @@
 namespace m26b {
 
 // ---- weight image ------------------------------------------------------------------------------------------------
-// payload [m_pairs][256 rows][k_pad / 2]: rows of two consecutive 128-row tiles, or (gated) 128 gate rows, then the up rows of
-// the same 128 features. Rows beyond n and columns beyond k are zero.
-// scales  [m_pairs][chunks][2][512]; gated: [m_pairs][2 halves][chunks][512], rows 0..63 of a block gate, 64..127 up.
+// payload [tiles][128 rows][k_pad / 2], scales [tiles][chunks][512]. A tile is 128 consecutive output features; for the gated form
+// it is 64 features, sixteen gate rows and then the sixteen up rows of the same features in every 32 (the lanes one warp reads
+// from tensor memory), so that a feature's gate and up meet by one shuffle. Rows beyond n and columns beyond k are zero; the
+// number of tiles is even.
 struct LinearSrc { const uint8_t *w[2], *s[2]; };    // gate / up, or one matrix
 
+// Which matrix and which of its features image row `row` holds.
+__device__ __forceinline__ void image_row(uint64_t row, int gated, int& matrix, uint64_t& feat) {
+    matrix = gated ? int((row >> 4) & 1) : 0;
+    feat = gated ? (row >> 5) * 16 + (row & 15) : row;
+}
 __global__ void __launch_bounds__(256) linear_prep_payload_kernel(LinearSrc src, int gated, uint32_t n, uint32_t k, uint32_t k_pad, uint64_t rows,
                                                                   uint8_t* __restrict__ dst) {
     const uint64_t vec_per_row = k_pad / 32, total = rows * vec_per_row;
     for (uint64_t i = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += uint64_t(gridDim.x) * blockDim.x) {
-        const uint64_t v = i % vec_per_row, row = i / vec_per_row;
-        const int m = gated ? int((row >> 7) & 1) : 0;
-        const uint64_t feat = gated ? (row >> 8) * 128 + (row & 127) : row;
+        const uint64_t v = i % vec_per_row;
+        int m;
+        uint64_t feat;
+        image_row(i / vec_per_row, gated, m, feat);
         uint32_t o[4] = {0, 0, 0, 0};
         if (feat < n && v * 32 < k) {
-            const uint8_t* from = src.w[m] + feat * (k / 2) + v * 16;
+            const uint8_t* from = (m ? src.w[1] : src.w[0]) + feat * (k / 2) + v * 16;
+            if ((reinterpret_cast<uintptr_t>(from) & 15) == 0) {
+                const uint4 a = *reinterpret_cast<const uint4*>(from);
+                o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w;
+            } else {
 #pragma unroll
-            for (int b = 0; b < 16; ++b) o[b >> 2] |= uint32_t(from[b]) << (8 * (b & 3));   // the source may have any alignment
+                for (int b = 0; b < 16; ++b) o[b >> 2] |= uint32_t(from[b]) << (8 * (b & 3));
+            }
         }
         reinterpret_cast<uint4*>(dst)[i] = make_uint4(o[0], o[1], o[2], o[3]);
     }
@@ -49,21 +60,12 @@ __global__ void __launch_bounds__(256) linear_prep_scales_kernel(LinearSrc src, 
                                                                  uint8_t* __restrict__ dst) {
     for (uint64_t i = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += uint64_t(gridDim.x) * blockDim.x) {
         const uint32_t o = uint32_t(i % kScaleBlockBytes);
-        const uint32_t r = (o >> 4) + 32u * ((o >> 2) & 3u), kb = o & 3u;
-        uint64_t feat, c;
-        int m = 0;
-        if (gated) {
-            c = (i / kScaleBlockBytes) % chunks;
-            const uint64_t ph = i / kScaleBlockBytes / chunks;                 // pair * 2 + half
-            feat = (ph >> 1) * 128 + (ph & 1) * 64 + (r & 63u);
-            m = int(r >> 6);
-        } else {
-            c = (i / kScaleBlockBytes / 2) % chunks;
-            feat = (i / kScaleBlockBytes / 2 / chunks) * 256 + ((i / kScaleBlockBytes) & 1) * 128 + r;
-        }
-        const uint64_t kb_all = c * 4 + kb;
+        const uint64_t c = (i / kScaleBlockBytes) % chunks, kb = c * 4 + (o & 3u);
+        int m;
+        uint64_t feat;
+        image_row(i / kScaleBlockBytes / chunks * kTileM + (o >> 4) + 32u * ((o >> 2) & 3u), gated, m, feat);
         uint8_t v = 127;
-        if (feat < n && kb_all * 32 < k) v = src.s[m][feat * (k / 32) + kb_all];
+        if (feat < n && kb * 32 < k) v = (m ? src.s[1] : src.s[0])[feat * (k / 32) + kb];
         dst[i] = v == 255 ? 254 : v;                                           // the reserved byte, as in the layer image
     }
 }
@@ -208,6 +210,25 @@ __device__ __forceinline__ void store_y(const LinearArgs& p, uint32_t token, uin
     const uint64_t at = uint64_t(token) * p.y_pitch + col;
     if (p.y_f32) static_cast<float*>(p.y)[at] = v;
     else static_cast<uint16_t*>(p.y)[at] = uint16_t(bf16x2_rn(v, 0.0f));
+}
+// Sixteen finished accumulator columns (tokens from `token`, valid below `end`) of the lane's weight row. Gated: lanes 0..15 hold the
+// gate of sixteen features and lanes 16..31 their up; of every two tokens the lower half finishes the first, the upper the second.
+template <bool GATED>
+__device__ __forceinline__ void store_columns(const LinearArgs& p, const uint32_t (&r)[16], uint32_t token, uint32_t end, uint32_t feat, int lane) {
+    if constexpr (GATED) {
+        const bool upper = lane >= 16;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            const float other = __uint_as_float(__shfl_xor_sync(0xffffffffu, upper ? r[j] : r[j + 1], 16));
+            const float mine = __uint_as_float(upper ? r[j + 1] : r[j]);
+            const uint32_t t = token + j + (upper ? 1 : 0);
+            if (t < end && feat < p.n) store_y(p, t, feat, upper ? silu_gate(other, mine) : silu_gate(mine, other));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (token + j < end && feat < p.n) store_y(p, token + j, feat, __uint_as_float(r[j]));
+    }
 }
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
@@ -377,13 +398,8 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             auto weights = [&](uint32_t i, uint32_t st) {
                 const uint32_t c = c0 + i;
                 mbar_expect_tx(&s.full[st], tx);
-                if constexpr (GATED) {          // 64 gate rows, then the 64 up rows of the same features
-                    tma_load_3d(s.a[st], &map_w, int(c * kChunkK), int((tile & 1) * 64), int(tile >> 1) * 2, &s.full[st]);
-                    bulk_load(s.sfa[st], p.sfa + (uint64_t(tile) * p.chunks + c) * kScaleBlockBytes, kScaleBlockBytes, &s.full[st]);
-                } else {
-                    tma_load_2d(s.a[st], &map_w, int(c * kChunkK), int(tile * kTileM), &s.full[st]);
-                    bulk_load(s.sfa[st], p.sfa + ((uint64_t(tile >> 1) * p.chunks + c) * 2 + (tile & 1)) * kScaleBlockBytes, kScaleBlockBytes, &s.full[st]);
-                }
+                tma_load_2d(s.a[st], &map_w, int(c * kChunkK), int(tile * kTileM), &s.full[st]);
+                bulk_load(s.sfa[st], p.sfa + (uint64_t(tile) * p.chunks + c) * kScaleBlockBytes, kScaleBlockBytes, &s.full[st]);
             };
             // the weights depend on no earlier kernel: their first stages are requested before the stream's last one ends
             const uint32_t early = n_chunks < uint32_t(T::kStages) ? n_chunks : uint32_t(T::kStages);
@@ -475,10 +491,10 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             tc_fence_after();
             const uint32_t t_acc = tb + ((q * 32u) << 16);
             // owner of a row and its place there: features are dealt in equal runs, gate and up of a feature together
-            const uint32_t log_run = (GATED ? 6 : 7) - log_split, f = GATED ? row & 63u : row;
-            const uint32_t owner = f >> log_run, slot = (f & ((1u << log_run) - 1)) + (GATED ? (row >> 6) << log_run : 0);
+            const uint32_t log_run = (GATED ? 6 : 7) - log_split, f = GATED ? q * 16 + (lane & 15) : row;
+            const uint32_t owner = f >> log_run, slot = (f & ((1u << log_run) - 1)) + (GATED ? uint32_t(lane >> 4) << log_run : 0);
             const uint32_t base = (split > 1 ? cluster_map(smem_u32(s.red), owner) : smem_u32(s.red)) + slot * 4;
-            const uint32_t feat = tile * kTileM + row;
+            const uint32_t feat = tile * (GATED ? 64 : kTileM) + f;
             for (uint32_t col = uint32_t(warp - 2) / 4 * 16; col < n_mma; col += 32) {
                 uint32_t r[16];
                 tmem_ld16(t_acc + col, r);
@@ -491,10 +507,8 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 } else {
                     tmem_wait_ld();
                 }
-                if (!GATED && split == 1) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (col + j < n_valid && feat < p.n) store_y(p, tok0 + col + j, feat, __uint_as_float(r[j]));
+                if (split == 1) {
+                    store_columns<GATED>(p, r, tok0 + col, tok0 + n_valid, feat, lane);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
@@ -506,7 +520,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     }
     if (split > 1) cluster_sync_all();
     else __syncthreads();
-    if (GATED || split > 1) {
+    if (split > 1) {
         // -------------------------------------------------------- epilogue, second half: partial sums in rank order
         const uint32_t log_feats = (GATED ? 6 : 7) - log_split, feats = 1u << log_feats;
         const uint32_t feat0 = tile * (GATED ? 64 : kTileM) + rank * feats;
@@ -523,6 +537,192 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         }
     }
     if (warp == 1) tmem_dealloc(s.tmem_base, T::kCols);
+}
+
+// ---- the product on CTA pairs (prefill) -----------------------------------------------------------------------------
+// cta_group::2: two CTAs of a cluster run one MMA of M = 256 (128 weight rows each) x N = up to 256 tokens, half of the token rows in
+// each CTA's shared memory. What bounds a block-scaled MMA at prefill is shared memory, which feeds the operands (128 B/clk) and
+// takes the loads: per 128-wide chunk and CTA this shape reads PIECES x 32 KB and fills 16 + PIECES x 16 KB in PIECES x 512 cycles of
+// math, 112 B/clk with two pieces; 128 tokens wide it would be 144, a single CTA of 128 x 128 tokens 192. The pieces
+// accumulate one after the other into the same 256 columns, which leaves the other half of tensor memory to the scales.
+// The accumulators are pulled into registers (64 per thread) and handed back before the epilogue's math, so that the next
+// item's MMAs run meanwhile. Barriers as in gemm_mx_pair.cuh: loads of both CTAs report to the first CTA's `full`.
+constexpr uint32_t kLpTokens = 256;
+constexpr int kLpEpiWarps = 16, kLpThreads = 64 + 32 * kLpEpiWarps;
+constexpr uint32_t kLpSfSlots = 8, kLpSfStride = 32;       // scale slots above the accumulators: 4 columns of weights, 8 per piece of tokens
+
+struct LinearPairMaps {
+    CUtensorMap w;          // weight rows, box 128
+    CUtensorMap tok[5];     // token rows, boxes of 128 / 64 / 32 / 16 / 8
+    CUtensorMap sfa;        // weight scale blocks as rows of 128 u32, box 1
+    CUtensorMap sfb;        // token scale blocks, box PIECES
+};
+template <int PIECES>
+struct LinearPairSmem {
+    static constexpr int kStages = PIECES == 2 ? 4 : 6;
+    alignas(1024) uint8_t a[kStages][kTileM * 128];
+    alignas(1024) uint8_t b[kStages][PIECES * (kLpTokens / 2) * 128];
+    alignas(128) uint8_t sfa[kStages][kScaleBlockBytes];
+    alignas(128) uint8_t sfb[kStages][2 * PIECES * kScaleBlockBytes];       // [128-token half of the tile][piece]
+    uint64_t full[kStages], empty[kStages], acc_full, acc_empty;
+    uint32_t tmem_base, abort_flag;
+};
+static_assert(sizeof(LinearPairSmem<2>) + 1024 <= 232448 && sizeof(LinearPairSmem<1>) + 1024 <= 232448, "a CTA has at most 227 KB of shared memory");
+
+// Items: 256 image rows x 256 tokens, the weight rows running fastest, strided over the pairs of the grid.
+template <int PIECES, bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
+linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs p, const uint32_t m_pairs, const uint32_t n_items) {
+    using Smem = LinearPairSmem<PIECES>;
+    constexpr uint32_t kStages = Smem::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const uint32_t pair_id = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+    volatile uint32_t* abort_flag = &s.abort_flag;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < kStages; ++i) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 1); }
+        mbar_init(&s.acc_full, 1);
+        mbar_init(&s.acc_empty, 2 * kLpEpiWarps);
+        s.abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == 1) { tmem_alloc_pair(&s.tmem_base, kTmemCols); tmem_relinquish_pair(); }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();          // the partner's barriers exist before anything arrives on them
+    tc_fence_after();
+    grid_dep_launch();
+    const uint32_t tb = s.tmem_base;
+    const auto tile_tokens = [&](uint32_t t) { const uint32_t left = p.rows - t * kLpTokens; return left < kLpTokens ? left : kLpTokens; };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ producer (both CTAs)
+        if (elect_one()) {
+            tma_prefetch_desc(&maps.w);
+            uint32_t stage = 0, phase = 0, issued = 0;
+            bool ok = true;
+            for (uint32_t it = pair_id; it < n_items && ok; it += n_pairs) {
+                const uint32_t m = it % m_pairs, t = it / m_pairs;
+                const uint32_t n_mma = (tile_tokens(t) + 15) & ~15u, half = n_mma >> 1, sf_tiles = n_mma > 128 ? 2 : 1;
+                const uint32_t tile = 2 * m + rank;
+                const uint32_t tx = kTileM * 64 + PIECES * half * 128 + kScaleBlockBytes + sf_tiles * PIECES * kScaleBlockBytes;
+                const auto weights = [&](uint32_t c, uint32_t st) {
+                    const uint32_t bar = cluster_map(smem_u32(&s.full[st]), 0);
+                    if (rank == 0) mbar_expect_tx(&s.full[st], 2 * tx);        // the bytes of both CTAs' loads
+                    tma_load_2d_pair(s.a[st], &maps.w, int(c * kChunkK), int(tile * kTileM), bar);
+                    tma_load_2d_pair(s.sfa[st], &maps.sfa, 0, int(tile * p.chunks + c), bar);
+                };
+                // the weights depend on no earlier kernel: the first stages' are requested before the stream's last one ends
+                uint32_t early = 0;
+                if (it == pair_id) {
+                    early = p.chunks < kStages ? p.chunks : kStages;
+                    for (uint32_t c = 0; c < early; ++c) weights(c, c);
+                    grid_dep_wait();
+                }
+                for (uint32_t c = 0; c < p.chunks; ++c) {
+                    if (c >= early) {
+                        if (!mbar_wait(&s.empty[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
+                        weights(c, stage);
+                    }
+                    const uint32_t bar = cluster_map(smem_u32(&s.full[stage]), 0);
+#pragma unroll
+                    for (uint32_t piece = 0; piece < PIECES; ++piece) {
+                        uint32_t r = 0;
+#pragma unroll
+                        for (uint32_t b = 0; b < 5; ++b) {
+                            const uint32_t box = 128u >> b;
+                            if (half - r >= box) {
+                                tma_load_2d_pair(s.b[stage] + (piece * (kLpTokens / 2) + r) * 128, &maps.tok[b], int(c * kChunkK),
+                                                 int(piece * p.rows_cap + t * kLpTokens + rank * half + r), bar);
+                                r += box;
+                            }
+                        }
+                    }
+                    for (uint32_t h = 0; h < sf_tiles; ++h)
+                        tma_load_2d_pair(s.sfb[stage] + h * PIECES * kScaleBlockBytes, &maps.sfb, 0, int(((2 * t + h) * p.chunks + c) * PIECES), bar);
+                    ++issued;
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
+            if (!ok) atomicOr(p.fault, uint32_t(kFaultPipeline));
+            if (*abort_flag && rank == 0) {        // a wait ran out: give the loads under way time to land
+                const long long t0 = clock64();
+                for (uint32_t i = 0; i < kStages && i < issued; ++i)
+                    while (!mbar_try_wait(&s.full[i], phase ^ (i < stage ? 0u : 1u)) && clock64() - t0 < kWaitCycles) {}
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issue (first CTA of the pair only)
+        if (rank == 0 && elect_one()) {
+            uint32_t stage = 0, phase = 0, local = 0, slot = 0;
+            bool ok = true;
+            const uint64_t a_desc0 = desc_sw128(smem_u32(s.a[0])), b_desc0 = desc_sw128(smem_u32(s.b[0]));
+            const uint64_t sfa_desc0 = desc_scale_block(smem_u32(s.sfa[0])), sfb_desc0 = desc_scale_block(smem_u32(s.sfb[0]));
+            for (uint32_t it = pair_id; it < n_items && ok; it += n_pairs, ++local) {
+                const uint32_t n_mma = (tile_tokens(it / m_pairs) + 15) & ~15u;
+                const uint32_t idesc0 = idesc_mx_pair(kFmtE2M1, kFmtE4M3, n_mma, 0, 0);
+                if (!mbar_wait(&s.acc_empty, (local & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                for (uint32_t c = 0; c < p.chunks; ++c) {
+                    if (!mbar_wait(&s.full[stage], phase, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t t_sf = tb + kLpTokens + slot * kLpSfStride;
+                    slot = (slot + 1) % kLpSfSlots;
+                    tc_cp_scales_pair(t_sf, sfa_desc0 + stage * (sizeof(s.sfa[0]) >> 4));
+                    const uint64_t sfb_d = sfb_desc0 + stage * (sizeof(s.sfb[0]) >> 4);
+#pragma unroll
+                    for (uint32_t piece = 0; piece < PIECES; ++piece) {
+                        tc_cp_scales_pair(t_sf + 4 + 8 * piece, sfb_d + piece * (kScaleBlockBytes >> 4));
+                        if (n_mma > 128) tc_cp_scales_pair(t_sf + 8 + 8 * piece, sfb_d + (PIECES + piece) * (kScaleBlockBytes >> 4));
+                    }
+                    const uint64_t ad = a_desc0 + stage * (sizeof(s.a[0]) >> 4), bd = b_desc0 + stage * (sizeof(s.b[0]) >> 4);
+#pragma unroll
+                    for (uint32_t piece = 0; piece < PIECES; ++piece)
+#pragma unroll
+                        for (uint32_t kb = 0; kb < 4; ++kb)
+                            tc_mma_mx_pair(tb, ad + 2 * kb, bd + piece * (((kLpTokens / 2) * 128) >> 4) + 2 * kb, idesc0 | (kb << 4) | (kb << 29), t_sf,
+                                           t_sf + 4 + 8 * piece, (c | piece | kb) ? 1u : 0u);
+                    tc_commit_pair(&s.empty[stage]);
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                }
+                if (ok) tc_commit_pair(&s.acc_full);
+            }
+            if (!ok) atomicOr(p.fault, uint32_t(kFaultPipeline));
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue (both CTAs)
+        const uint32_t q = uint32_t(warp) & 3u, col0 = uint32_t(warp - 2) / 4 * 64;      // lane quadrant, first of the warp's 64 tokens
+        const uint32_t t_acc = tb + ((q * 32u) << 16) + col0;
+        uint32_t local = 0;
+        for (uint32_t it = pair_id; it < n_items; it += n_pairs, ++local) {
+            const uint32_t m = it % m_pairs, t = it / m_pairs, n_valid = tile_tokens(t), n_mma = (n_valid + 15) & ~15u;
+            const bool got = mbar_wait(&s.acc_full, local & 1u, abort_flag);
+            if (!__all_sync(0xffffffffu, got)) {
+                if (lane == 0) atomicOr(p.fault, uint32_t(kFaultPipeline));
+                break;
+            }
+            tc_fence_after();
+            uint32_t r[4][16];
+#pragma unroll
+            for (uint32_t g = 0; g < 4; ++g)
+                if (col0 + 16 * g < n_mma) tmem_ld16(t_acc + 16 * g, r[g]);
+            tmem_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(cluster_map(smem_u32(&s.acc_empty), 0));
+            const uint32_t tile = 2 * m + rank, feat = GATED ? tile * 64 + q * 16 + (lane & 15) : tile * kTileM + q * 32 + lane;
+#pragma unroll
+            for (uint32_t g = 0; g < 4; ++g)
+                if (col0 + 16 * g < n_valid) store_columns<GATED>(p, r[g], t * kLpTokens + col0 + 16 * g, t * kLpTokens + n_valid, feat, lane);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();          // nothing of either CTA is torn down while the partner may still signal it
+    if (warp == 1) tmem_dealloc_pair(tb, kTmemCols);
 }
 
 }  // namespace m26b

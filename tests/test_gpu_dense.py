@@ -183,6 +183,51 @@ def test_quantised_activations(torch, rows, gated):
     check(torch, run(q, rows, x_scales=xs), y, rounded(y, bound, False))
 
 
+@pytest.mark.parametrize("rows", [129, 136, 150, 256, 257, 273, 384, 385, 400, 511, 512, 700])
+@pytest.mark.parametrize("k", [32, 160, 1152])
+def test_enough_work_for_cta_pairs(torch, rows, k):
+    """At least a quarter as many 256-row x 256-token items as SMs: linear and gated, both kinds of activations, both output types."""
+    import mimo26f_afd_b200 as M
+
+    g = gen(torch, rows + k)
+    n = 9601
+    w, s = make_weights(torch, n, k, g)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(torch.bfloat16)
+    q = torch.randint(0, 127, (rows, k), dtype=torch.uint8, device="cuda", generator=g)
+    xs = torch.randint(112, 118, (rows, k // 32), dtype=torch.uint8, device="cuda", generator=g)
+    W = weight_f64(torch, w, s)
+    run = Runner(torch, M.Linear.new(w, s, n, k), rows)
+    y, bound = product_and_bound(torch, x.double(), W)
+    check(torch, run(x, rows), y, rounded(y, bound, False))
+    yq, bq = product_and_bound(torch, e4m3_f64(torch, q, xs), W, quantised=True)
+    check(torch, run(q, rows, x_scales=xs, f32=False), yq, rounded(yq, bq, True))
+    half = n // 2
+    gated = Runner(torch, M.Linear.gated(w[:half].contiguous(), s[:half].contiguous(), w[half:2 * half].contiguous(), s[half:2 * half].contiguous(), half, k), rows)
+    for a, da, got in ((y, bound, gated(x, rows, f32=False)), (yq, bq, gated(q, rows, x_scales=xs, f32=False))):
+        b, db, a, da = a[:, half:2 * half], da[:, half:2 * half], a[:, :half], da[:, :half]
+        silu = a * torch.sigmoid(a)
+        check(torch, got, silu * b, rounded(silu * b, 1.1 * da * (b.abs() + db) + silu.abs() * db + 2.0**-19 * (silu * b).abs(), True))
+    assert int(run.fault) == 0 and int(gated.fault) == 0
+
+
+def test_cta_pairs_with_many_items_each(torch):
+    import mimo26f_afd_b200 as M
+
+    n, k, rows = 4096, 2048, 4000
+    g = gen(torch, 77)
+    w, s = make_weights(torch, n, k, g)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(torch.bfloat16)
+    run = Runner(torch, M.Linear.new(w, s, n, k), rows)
+    y, bound = product_and_bound(torch, x.double(), weight_f64(torch, w, s))
+    a = run(x, rows).clone()
+    check(torch, a, y, rounded(y, bound, False))
+    x2 = x.clone()
+    x2[1::2] = x[0::2]
+    b = run(x2, rows)
+    torch.cuda.synchronize()
+    assert torch.equal(a[0::2], b[0::2]) and int(run.fault) == 0
+
+
 def test_bf16_activations_pass_unquantised(torch):
     """One weight of 1.0 per row: the output is the activation itself, bit for bit down to 2^-14 of its block's largest."""
     import mimo26f_afd_b200 as M
