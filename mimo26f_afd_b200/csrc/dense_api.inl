@@ -178,30 +178,73 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
 }
 
 // Rows are strided over by as many CTAs as the GPU holds at once.
-template <int VEC, int PER, int MAX_THREADS, bool Y32, bool H32>
-cudaError_t launch_norm_kernel(const NormArgs& a, uint32_t threads, cudaStream_t st) {
-    const auto kernel = block_norm_kernel<VEC, PER, MAX_THREADS, Y32, H32>;
-    static const int sms = [] { int dev = 0, n = 148; cudaGetDevice(&dev); cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev); return n; }();
-    static std::atomic<int> resident[33]{};                            // CTAs per SM by warps per CTA
-    const uint32_t block = MAX_THREADS == 128 ? 128u : threads;
-    int per_sm = resident[block / 32].load(std::memory_order_relaxed);
-    if (!per_sm) {
-        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, int(block), 0);
+template <int VEC, int PER, int THREADS, bool Y32, bool H32, bool GATE_ELEM>
+cudaError_t launch_norm_kernel(const NormArgs& a, cudaStream_t st) {
+    const auto kernel = block_norm_kernel<VEC, PER, THREADS, Y32, H32, GATE_ELEM>;
+    constexpr uint32_t block = THREADS == 32 ? 128 : THREADS;
+    static std::atomic<uint32_t> known{0};                             // CTAs the device holds: the same for every GPU of the box
+    uint32_t room = known.load(std::memory_order_relaxed);
+    if (!room) {
+        int dev = 0, sms = 0, per_sm = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, int(block), 0);
         if (e != cudaSuccess || per_sm < 1) return e != cudaSuccess ? e : cudaErrorLaunchOutOfResources;
-        resident[block / 32].store(per_sm, std::memory_order_relaxed);
+        room = uint32_t(sms * per_sm);
+        known.store(room, std::memory_order_relaxed);
     }
-    const uint32_t need = MAX_THREADS == 128 ? (a.rows + 3) / 4 : a.rows, room = uint32_t(sms * per_sm);
+    const uint32_t need = THREADS == 32 ? (a.rows + 3) / 4 : a.rows;
     return launch_dependent(kernel, need < room ? need : room, block, 0, st, a);
 }
-template <int VEC, int PER, int MAX_THREADS>
+template <int VEC, int PER, int THREADS>
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
-    const uint32_t threads = ((a.width + VEC * PER - 1) / (VEC * PER) + 31) & ~31u;
-    if (threads == 32) {
-        if (a.y_f32) return a.h_f32 ? launch_norm_kernel<VEC, PER, 128, true, true>(a, threads, st) : launch_norm_kernel<VEC, PER, 128, true, false>(a, threads, st);
-        return a.h_f32 ? launch_norm_kernel<VEC, PER, 128, false, true>(a, threads, st) : launch_norm_kernel<VEC, PER, 128, false, false>(a, threads, st);
+    const auto typed = [&](auto y32, auto h32) {
+        if (a.gate_kind == kGateElement) return launch_norm_kernel<VEC, PER, THREADS, y32.value, h32.value, true>(a, st);
+        return launch_norm_kernel<VEC, PER, THREADS, y32.value, h32.value, false>(a, st);
+    };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    if (a.y_f32) return a.h_f32 ? typed(yes, yes) : typed(yes, no);
+    return a.h_f32 ? typed(no, yes) : typed(no, no);
+}
+// Threads and vectors per thread by width: a row's CTA is as small as its registers allow (8,192 x 4,096: 62 us with two vectors of
+// eight in each of 256 threads, 87 with one in 512, 72 with four in 128), since what a row costs beyond its bytes is two
+// reductions over its threads. Wider rows than 8,192 do not fit the registers of a CTA and take block_norm_any_kernel.
+cudaError_t launch_norm_vec8(const NormArgs& a, cudaStream_t st) {
+    if (a.width <= 512) return launch_norm<8, 2, 32>(a, st);
+    if (a.width <= 1024) return launch_norm<8, 2, 64>(a, st);
+    if (a.width <= 2048) return launch_norm<8, 2, 128>(a, st);
+    if (a.width <= 4096) return launch_norm<8, 2, 256>(a, st);
+    return launch_norm<8, 2, 512>(a, st);
+}
+cudaError_t launch_norm_vec4(const NormArgs& a, cudaStream_t st) {
+    if (a.width <= 1024) return launch_norm<4, 4, 64>(a, st);
+    if (a.width <= 4096) return launch_norm<4, 4, 256>(a, st);
+    return launch_norm<4, 4, 512>(a, st);
+}
+template <uint32_t T, bool Y32, bool H32>
+cudaError_t launch_norm_any(const NormArgs& a, cudaStream_t st) {
+    const auto kernel = block_norm_any_kernel<T, Y32, H32>;
+    const size_t smem = size_t(a.width) * 4;
+    static std::atomic<uint64_t> opted{0};                             // one flag bit per device of this process
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(opted.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kNormMaxWidth) * 4);
+        if (e != cudaSuccess) return e;
+        opted.fetch_or(bit, std::memory_order_relaxed);
     }
-    if (a.y_f32) return a.h_f32 ? launch_norm_kernel<VEC, PER, MAX_THREADS, true, true>(a, threads, st) : launch_norm_kernel<VEC, PER, MAX_THREADS, true, false>(a, threads, st);
-    return a.h_f32 ? launch_norm_kernel<VEC, PER, MAX_THREADS, false, true>(a, threads, st) : launch_norm_kernel<VEC, PER, MAX_THREADS, false, false>(a, threads, st);
+    return launch_dependent(kernel, a.rows, T, smem, st, a);
+}
+template <bool Y32, bool H32>
+cudaError_t launch_norm_any_width(const NormArgs& a, cudaStream_t st) {
+    // many rows: CTAs so small that eight of them share an SM (8,192 x 4,095: 101 us, 178 with 1,024 threads); few rows: the threads
+    // of one SM on one row (1 x 4,095: 4.4 us, 7.0 with 256)
+    if (a.width <= 512) return launch_norm_any<64, Y32, H32>(a, st);
+    if (a.width <= 1024 || (a.width <= 8192 && a.rows > 296)) return launch_norm_any<256, Y32, H32>(a, st);
+    return launch_norm_any<1024, Y32, H32>(a, st);
 }
 
 }  // namespace
@@ -281,10 +324,10 @@ int m26b_block_norm_dev(const m26b_block_norm_args* args, void* stream, char* er
     const uint64_t y_pitch = in.y_pitch ? in.y_pitch : width, h_pitch = in.h_pitch ? in.h_pitch : width, n_pitch = in.n_pitch ? in.n_pitch : width;
     if (y_pitch < width || h_pitch < width || n_pitch < width) { set_msg(err, errlen, "m26b block norm: a pitch is below the width"); return 1; }
     NormArgs a{};
-    uintptr_t vec = 0, elem = 0;                      // address bits that keep 16-byte vectors / single elements from being aligned
+    uintptr_t vec8 = 0, vec4 = 0, elem = 0;           // address bits that keep vectors of 8 / of 4 / single elements from being aligned
     const auto see = [&](const void* p, int f32) {
         const uintptr_t v = reinterpret_cast<uintptr_t>(p);
-        vec |= v & 15; elem |= v & (f32 ? 3 : 1);
+        vec8 |= v & 15; vec4 |= v & (f32 ? 15 : 7); elem |= v & (f32 ? 3 : 1);
     };
     for (int r = 0; r < n_planes; ++r) {
         if (!in.planes[r]) { set_msg(err, errlen, "m26b block norm: bad arguments"); return 1; }
@@ -305,17 +348,12 @@ int m26b_block_norm_dev(const m26b_block_norm_args* args, void* stream, char* er
     if (elem) { set_msg(err, errlen, "m26b block norm: a pointer is not aligned to its element size"); return 1; }
     if (!rows) return 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const uint64_t pitches = (n_planes ? y_pitch : 0) | (in.residual || in.h_out ? h_pitch : 0) | (in.n_out ? n_pitch : 0);
     cudaError_t e;
-    if (!vec && (width | (n_planes ? y_pitch : 0) | (in.residual || in.h_out ? h_pitch : 0) | (in.n_out ? n_pitch : 0)) % 8 == 0) {
-        if (width <= 2048) e = launch_norm<8, 1, 256>(a, st);
-        else if (width <= 8192) e = launch_norm<8, 2, 512>(a, st);
-        else if (width <= 16384) e = launch_norm<8, 2, 1024>(a, st);
-        else e = launch_norm<8, 4, 1024>(a, st);
-    } else {
-        if (width <= 8192) e = launch_norm<1, 8, 1024>(a, st);
-        else if (width <= 16384) e = launch_norm<1, 16, 1024>(a, st);
-        else e = launch_norm<1, 32, 1024>(a, st);
-    }
+    if (!vec8 && (width | pitches) % 8 == 0 && width <= 8192) e = launch_norm_vec8(a, st);
+    else if (!vec4 && pitches % 4 == 0 && width <= 8192) e = launch_norm_vec4(a, st);
+    else if (y_dtype) e = h_dtype ? launch_norm_any_width<true, true>(a, st) : launch_norm_any_width<true, false>(a, st);
+    else e = h_dtype ? launch_norm_any_width<false, true>(a, st) : launch_norm_any_width<false, false>(a, st);
     if (e != cudaSuccess) { cudaGetLastError(); set_err(err, errlen, "m26b block norm launch", e); return 2; }
     return 0;
 }

@@ -506,6 +506,14 @@ def test_norm_widths(torch, rows, width):
     norm_case(torch, rows, width)
 
 
+@pytest.mark.parametrize("width", [1, 2, 3, 5, 63, 255, 257, 1021, 1027, 4093, 4095, 5001, 8191, 16381, 20003, 32765])
+@pytest.mark.parametrize("planes,kind", [(1, 3), (4, 1)])
+def test_norm_odd_widths_in_aligned_rows(torch, width, planes, kind):
+    """Rows on vector boundaries whose last vector is short."""
+    norm_case(torch, 5, width, planes=planes, kind=kind, pad=-width % 4)
+    norm_case(torch, 3, width, planes=planes, kind=kind, pad=-width % 8, h32=False, n32=False, w32=False)
+
+
 @pytest.mark.parametrize("y32", [False, True])
 @pytest.mark.parametrize("h32", [False, True])
 @pytest.mark.parametrize("n32,w32", [(False, True), (True, False), (False, False)])
@@ -529,7 +537,7 @@ def test_norm_planes(torch, planes):
     norm_case(torch, 4, 770, planes=planes, post=planes > 0)
 
 
-@pytest.mark.parametrize("pad,off", [(0, 0), (8, 8), (3, 0), (0, 1), (16, 4)])
+@pytest.mark.parametrize("pad,off", [(0, 0), (8, 8), (3, 0), (0, 1), (16, 4), (4, 0)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_norm_strides_alignment_and_in_place(torch, pad, off, in_place):
     for h32 in (True, False):
