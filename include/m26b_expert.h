@@ -355,28 +355,35 @@ int m26b_plan_static(const int32_t* ids, const float* weights, uint32_t rows, in
  *              waits for all work queued on the current device; the sources may be freed when it returns.
  *   new_gated: the same for gate_proj and up_proj, both [n][k].
  *   workspace_bytes: device bytes m26b_linear_dev needs for `rows` tokens (0 for 0 rows); grows with rows up to 8,192.
- *   linear_dev: x [rows][k] with rows x_pitch elements apart, x_dtype 0 = BF16 or 2 = E4M3 with x_scales u8 [rows][k/32]
- *              (UE8M0, dense) -> y [rows][n] with rows y_pitch elements apart, y_dtype 0 = BF16 (one rounding, nearest even) or
- *              1 = FP32. A pitch of 0 means dense rows. Only y's n columns of `rows` rows are written. Any number of rows: one
- *              token to a prefill batch (passes of 8,192); 0 rows is no work. BF16 activations are not quantised: a K32 block
- *              enters the product as two E4M3 pieces that equal it exactly, save for elements below 2^-14 of the block's
- *              largest, which carry an error of at most 2^-21 of that largest. Products accumulate in FP32. A row with an
- *              infinity, a NaN (or, for x_dtype 2, a NaN code or scale byte 255) in it is NaN in all its outputs. A row's
- *              result does not change with the other rows' values.
- *              workspace: 128-byte aligned device memory of at least workspace_bytes(rows), one call at a time (calls that
- *              may overlap, or captured graphs that may run together, each need their own); its content is of no use between
- *              calls. fault_dev: one u32 that receives code 3 (ORed) if a bounded wait inside the kernel ran out, in which
- *              case y is undefined. Nothing is allocated, nothing is synchronised, and a call can be captured into a graph;
- *              the handle must stay alive until the work is done. Enqueued on `stream` (NULL = the default stream). */
+ *   linear_dev: x [rows][k], BF16 or E4M3 with UE8M0 scales per 32 k -> y [rows][n], BF16 (one rounding, nearest even) or
+ *              FP32. Only y's n columns of `rows` rows are written. Any number of rows: one token to a prefill batch (passes of
+ *              8,192); 0 rows is no work. BF16 activations are not quantised: a K32 block enters the product as two E4M3
+ *              pieces that equal it exactly, save for elements below 2^-14 of the block's largest, which carry an error of
+ *              at most 2^-21 of that largest. Products accumulate in FP32. A row with an infinity, a NaN (or, for E4M3, a NaN
+ *              code or scale byte 255) in it is NaN in all its outputs. A row's result does not change with the other rows'
+ *              values. Nothing is allocated, nothing is synchronised, and a call can be captured into a graph; the handle
+ *              must stay alive until the work is done, the argument record is read before the call returns. Enqueued on
+ *              `stream` (NULL = the default stream). */
 typedef struct m26b_linear m26b_linear;
 int m26b_linear_new(const uint8_t* w, const uint8_t* s, uint32_t n, uint32_t k, m26b_linear** out, char* err, size_t errlen);
 int m26b_linear_new_gated(const uint8_t* gate_w, const uint8_t* gate_s, const uint8_t* up_w, const uint8_t* up_s, uint32_t n, uint32_t k,
                           m26b_linear** out, char* err, size_t errlen);
 void m26b_linear_free(m26b_linear* l);
 uint64_t m26b_linear_workspace_bytes(const m26b_linear* l, uint32_t rows);
-int m26b_linear_dev(const m26b_linear* l, const void* x, int x_dtype, const uint8_t* x_scales, uint64_t x_pitch, uint32_t rows, void* y,
-                    int y_dtype, uint64_t y_pitch, void* workspace, uint64_t workspace_bytes, uint32_t* fault_dev, void* stream, char* err,
-                    size_t errlen);
+typedef struct m26b_linear_args {
+    const void* x;              /* device [rows][k], rows x_pitch elements apart (0: dense) */
+    const uint8_t* x_scales;    /* x_dtype 2: device [rows][k/32] UE8M0, dense; else unused */
+    void* y;                    /* device [rows][n], rows y_pitch elements apart (0: dense) */
+    void* workspace;            /* device, 128-byte aligned, at least m26b_linear_workspace_bytes(rows). One call at a time: calls that */
+    uint64_t workspace_bytes;   /* may overlap, or captured graphs that may run together, each need their own. No use between calls. */
+    uint32_t* fault_dev;        /* receives code 3 (ORed) if a bounded wait inside the kernel ran out; y is undefined then */
+    uint64_t x_pitch, y_pitch;
+    uint32_t rows;
+    int32_t x_dtype;            /* 0 BF16, 2 E4M3 */
+    int32_t y_dtype;            /* 0 BF16, 1 FP32 */
+    int32_t reserved;           /* 0 */
+} m26b_linear_args;
+int m26b_linear_dev(const m26b_linear* l, const m26b_linear_args* args, void* stream, char* err, size_t errlen);
 
 /* The step between two blocks in one pass over each row [width] (1..32,768), m26b_rank_sum_residual_dev with the norms around it:
  *   u = planes[0] + planes[1] + ...            rank order, FP32

@@ -271,25 +271,25 @@ uint64_t m26b_linear_workspace_bytes(const m26b_linear* l, uint32_t rows) {
     const uint64_t cap = linear_rows_cap(rows);
     return 2 * (cap * l->k_pad + (cap + 127) / 128 * (l->k_pad / kChunkK) * kScaleBlockBytes);
 }
-int m26b_linear_dev(const m26b_linear* l, const void* x, int x_dtype, const uint8_t* x_scales, uint64_t x_pitch, uint32_t rows, void* y,
-                    int y_dtype, uint64_t y_pitch, void* workspace, uint64_t workspace_bytes, uint32_t* fault_dev, void* stream, char* err,
-                    size_t errlen) {
-    if (!l || !(x_dtype == 0 || x_dtype == 2) || y_dtype < 0 || y_dtype > 1) {
+int m26b_linear_dev(const m26b_linear* l, const m26b_linear_args* args, void* stream, char* err, size_t errlen) {
+    if (!l || !args || !(args->x_dtype == 0 || args->x_dtype == 2) || args->y_dtype < 0 || args->y_dtype > 1 || args->reserved) {
         set_msg(err, errlen, "m26b linear: bad handle/dtype (x 0 BF16 or 2 E4M3, y 0 BF16 or 1 FP32)");
         return 1;
     }
+    const m26b_linear_args& in = *args;
+    const uint32_t rows = in.rows;
     if (!rows) return 0;
-    if (!x_pitch) x_pitch = l->k;
-    if (!y_pitch) y_pitch = l->n;
-    if (!x || !y || !fault_dev || (x_dtype == 2 && !x_scales) || x_pitch < l->k || y_pitch < l->n) {
+    const bool bf16 = in.x_dtype == 0;
+    const uint64_t x_pitch = in.x_pitch ? in.x_pitch : l->k, y_pitch = in.y_pitch ? in.y_pitch : l->n;
+    if (!in.x || !in.y || !in.fault_dev || (!bf16 && !in.x_scales) || x_pitch < l->k || y_pitch < l->n) {
         set_msg(err, errlen, "m26b linear: bad pointers/pitch");
         return 1;
     }
-    if ((x_dtype == 0 && reinterpret_cast<uintptr_t>(x) % 2) || reinterpret_cast<uintptr_t>(y) % (y_dtype ? 4 : 2)) {
+    if ((bf16 && reinterpret_cast<uintptr_t>(in.x) % 2) || reinterpret_cast<uintptr_t>(in.y) % (in.y_dtype ? 4 : 2)) {
         set_msg(err, errlen, "m26b linear: x or y is not aligned to its element size");
         return 1;
     }
-    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 128 || workspace_bytes < m26b_linear_workspace_bytes(l, rows)) {
+    if (!in.workspace || reinterpret_cast<uintptr_t>(in.workspace) % 128 || in.workspace_bytes < m26b_linear_workspace_bytes(l, rows)) {
         set_msg(err, errlen, "m26b linear: workspace too small or not 128-byte aligned (m26b_linear_workspace_bytes)");
         return 1;
     }
@@ -297,13 +297,14 @@ int m26b_linear_dev(const m26b_linear* l, const void* x, int x_dtype, const uint
     const cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) { set_err(err, errlen, "m26b linear device", e); return 2; }
     if (dev != l->device) { set_msg(err, errlen, "m26b linear: the handle belongs to another device"); return 1; }
-    const uint64_t x_row = x_pitch * (x_dtype == 0 ? 2 : 1), y_row = y_pitch * (y_dtype ? 4 : 2);
+    const uint64_t x_row = x_pitch * (bf16 ? 2 : 1), y_row = y_pitch * (in.y_dtype ? 4 : 2);
     for (uint32_t r0 = 0; r0 < rows; r0 += kLinearPassRows) {
         const uint32_t m = rows - r0 < kLinearPassRows ? rows - r0 : kLinearPassRows;
-        const int rc = linear_pass(l, static_cast<const uint8_t*>(x) + r0 * x_row, x_dtype == 0, x_scales ? x_scales + uint64_t(r0) * (l->k / kBlockK) : nullptr,
-                                   x_pitch, m, static_cast<uint8_t*>(y) + r0 * y_row, y_dtype, y_pitch, static_cast<uint8_t*>(workspace), fault_dev,
-                                   static_cast<cudaStream_t>(stream), err, errlen);
+        const int rc = linear_pass(l, static_cast<const uint8_t*>(in.x) + r0 * x_row, bf16, bf16 ? nullptr : in.x_scales + uint64_t(r0) * (l->k / kBlockK),
+                                   x_pitch, m, static_cast<uint8_t*>(in.y) + r0 * y_row, in.y_dtype, y_pitch, static_cast<uint8_t*>(in.workspace),
+                                   in.fault_dev, static_cast<cudaStream_t>(stream), err, errlen);
         if (rc) return rc;
+        if (rows - r0 <= kLinearPassRows) break;       // r0 must not pass 32 bits
     }
     return 0;
 }

@@ -19,7 +19,8 @@ GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_ELEMENT = 0, 1, 2, 3
 Y_BF16, Y_F32 = 0, 1
 
 
-# struct m26b_block_norm_args of the header
+# struct m26b_linear_args and struct m26b_block_norm_args of the header
+_LINEAR_ARGS = struct.Struct("@4PQP2QI3i")
 _NORM_ARGS = struct.Struct("@14P3Q3f2I7i")
 _local = threading.local()
 
@@ -93,9 +94,13 @@ def linear_dev(layer: Linear, x, rows: int, y, *, x_dtype: int = X_BF16, x_scale
     that receives code 3 if a bounded wait inside the kernel ran out."""
     if workspace_bytes is None:
         workspace_bytes = 0 if workspace is None else _nbytes(workspace)
+    try:
+        args = _LINEAR_ARGS.pack(_addr(x), _addr(x_scales), _addr(y), _addr(workspace), workspace_bytes, _addr(fault), x_pitch, y_pitch, rows,
+                                 x_dtype, y_dtype, 0)
+    except (struct.error, OverflowError) as e:        # a negative or oversized number
+        raise ExpertError(1, f"m26b linear: bad arguments ({e})") from None
     err = _err()
-    rc = _native.lib().m26b_linear_dev(layer._h, _addr(x), x_dtype, _addr(x_scales), x_pitch, rows, _addr(y), y_dtype, y_pitch, _addr(workspace),
-                                       workspace_bytes, _addr(fault), _addr(stream), err, 256)
+    rc = _native.lib().m26b_linear_dev(layer._h, args, _addr(stream), err, 256)
     if rc:
         _check(rc, err)
 
@@ -110,7 +115,7 @@ def block_norm_dev(planes, residual, rows: int, width: int, *, post_w=None, gate
     if n > 8:
         raise ExpertError(1, "m26b block norm: bad arguments")
     try:
-        args = _NORM_ARGS.pack(*[_addr(p) for p in planes], *_PAD[n], _addr(post_w), _addr(gate), _addr(residual), _addr(pre_w), _addr(h_out),
+        args = _NORM_ARGS.pack(*map(_addr, planes), *_PAD[n], _addr(post_w), _addr(gate), _addr(residual), _addr(pre_w), _addr(h_out),
                                _addr(n_out), y_pitch, h_pitch, n_pitch, y_scale, residual_scale, eps, rows, width, n, gate_kind, y_dtype, h_dtype,
                                n_dtype, w_dtype, 0)
     except (struct.error, OverflowError) as e:        # a negative or oversized number

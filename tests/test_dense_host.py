@@ -39,6 +39,42 @@ def test_block_norm_refuses(kw):
     assert e.value.code == 1 and "m26b block norm" in e.value.message
 
 
+@pytest.mark.parametrize("kw", [dict(rows=-1), dict(rows=1 << 32), dict(y_pitch=-64), dict(gate_kind=1 << 40)])
+def test_numbers_that_do_not_fit_the_record_are_refused(kw):
+    import mimo26f_afd_b200 as M
+
+    with pytest.raises(M.ExpertError) as e:
+        block_norm(**kw)
+    assert e.value.code == 1
+
+    class Handle:
+        _h = None
+
+    with pytest.raises(M.ExpertError) as e:
+        M.linear_dev(Handle(), P, kw.get("rows", -1), P)
+    assert e.value.code == 1
+
+
+def test_argument_records_match_the_header():
+    """Sizes of the packed records against the C structs, compiled here."""
+    import subprocess
+    import tempfile
+
+    from conftest import ROOT
+    from mimo26f_afd_b200 import dense
+
+    with tempfile.TemporaryDirectory() as d:
+        src = f'{d}/sizes.c'
+        with open(src, "w") as f:
+            f.write('#include <stdio.h>\n#include <stddef.h>\n#include "m26b_expert.h"\nint main(void) { printf("%zu %zu %zu %zu %zu %zu\\n", '
+                    'sizeof(m26b_linear_args), offsetof(m26b_linear_args, rows), offsetof(m26b_linear_args, x_pitch), '
+                    'sizeof(m26b_block_norm_args), offsetof(m26b_block_norm_args, y_scale), offsetof(m26b_block_norm_args, n_planes)); return 0; }')
+        subprocess.run(["gcc", "-I", f"{ROOT}/include", "-o", f"{d}/sizes", src], check=True)
+        got = [int(v) for v in subprocess.run([f"{d}/sizes"], check=True, capture_output=True, text=True).stdout.split()]
+    assert got[0] == (dense._LINEAR_ARGS.size + 7) // 8 * 8 and got[1] == 64 and got[2] == 48
+    assert got[3] == (dense._NORM_ARGS.size + 7) // 8 * 8 and got[4] == 14 * 8 + 3 * 8 and got[5] == got[4] + 20
+
+
 @pytest.mark.parametrize("n,k", [(0, 64), (64, 0), (64, 33), (64, 16), ((1 << 20) + 1, 64), (64, (1 << 20) + 32)])
 def test_linear_refuses_extents(n, k):
     import mimo26f_afd_b200 as M
@@ -60,7 +96,8 @@ def test_linear_refuses_null_tensors_and_handles():
         assert e.value.code == 1
     lib = _native.lib()
     err = ctypes.create_string_buffer(256)
-    assert lib.m26b_linear_dev(None, P, 0, None, 0, 1, P, 0, 0, P, 1 << 20, P, None, err, 256) == 1 and b"bad handle" in err.value
+    assert lib.m26b_linear_dev(None, b"\0" * 256, None, err, 256) == 1 and b"bad handle" in err.value
+    assert lib.m26b_block_norm_dev(None, None, err, 256) == 1 and b"bad arguments" in err.value
     assert lib.m26b_linear_workspace_bytes(None, 5) == 0
     lib.m26b_linear_free(None)
 
