@@ -16,7 +16,6 @@ namespace {
 
 constexpr uint32_t kLinearMaxDim = 1u << 20;
 constexpr uint32_t kLinearPassRows = 8192;      // tokens per pass: bounds the workspace at 2 x 8192 x k bytes
-constexpr uint32_t kLinearDirectRows = 32;      // requests up to this many tokens take aligned activations as they are
 
 int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool gated, uint32_t n, uint32_t k, m26b_linear** out, char* err,
                size_t errlen) {
@@ -63,6 +62,12 @@ int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool 
 
 uint32_t linear_rows_cap(uint32_t rows) { return ((rows < kLinearPassRows ? rows : kLinearPassRows) + 15) & ~15u; }
 
+// log2 of the CTAs that share a weight tile's K: doubled while the CTAs still fit the SMs at once and each keeps at least two chunks.
+uint32_t linear_log_split(uint64_t ctas, uint64_t room, uint32_t chunks) {
+    uint32_t log_split = 0;
+    while (log_split < 3 && (ctas << (log_split + 1)) <= room && chunks >= 4u << log_split) ++log_split;
+    return log_split;
+}
 template <int B_ROWS, int PIECES, bool GATED, bool DIRECT>
 cudaError_t launch_linear(const m26b_linear* L, const TokenMaps& mx, const LinearArgs& a, cudaStream_t st) {
     using T = LinearTile<B_ROWS, PIECES>;
@@ -76,11 +81,9 @@ cudaError_t launch_linear(const m26b_linear* L, const TokenMaps& mx, const Linea
         opted.fetch_or(bit, std::memory_order_relaxed);
     }
     const uint32_t feats = GATED ? 64 : kTileM, tiles = (a.n + feats - 1) / feats, tok_tiles = (a.rows + B_ROWS - 1) / B_ROWS;
-    // K is split over a cluster while the CTAs still fit the SMs at once and each keeps at least two chunks
-    uint32_t log_split = 0;
-    while (log_split < 3 && (uint64_t(tiles) * tok_tiles << (log_split + 1)) <= uint64_t(L->sms) * T::kCtasPerSm && a.chunks >= 4u << log_split) ++log_split;
+    const uint32_t log_split = linear_log_split(uint64_t(tiles) * tok_tiles, uint64_t(L->sms) * T::kCtasPerSm, a.chunks);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(tiles << log_split, tok_tiles); cfg.blockDim = dim3(kLinearThreads); cfg.dynamicSmemBytes = size_t(smem); cfg.stream = st;
+    cfg.gridDim = dim3(tiles << log_split, tok_tiles); cfg.blockDim = dim3(T::kThreads); cfg.dynamicSmemBytes = size_t(smem); cfg.stream = st;
     cudaLaunchAttribute at[2]{};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -120,18 +123,47 @@ int linear_pair_ctas(const m26b_linear* L) {
     return ctas;
 }
 template <int PIECES, bool GATED>
-cudaError_t launch_linear_pair(const m26b_linear* L, const LinearPairMaps& maps, const LinearArgs& a, cudaStream_t st) {
-    const uint32_t m_pairs = L->tiles / 2, items = m_pairs * ((a.rows + kLpTokens - 1) / kLpTokens);
+cudaError_t launch_linear_pair(const m26b_linear* L, const LinearPairMaps& maps, const LinearArgs& a, uint32_t tile, cudaStream_t st) {
+    const uint32_t m_pairs = L->tiles / 2, items = m_pairs * ((a.rows + tile - 1) / tile);
     const uint32_t room = uint32_t(linear_pair_ctas<PIECES, GATED>(L));
     return launch_dependent(linear_pair_kernel<PIECES, GATED>, 2 * items < room ? 2 * items : room, kLpThreads, sizeof(LinearPairSmem<PIECES>) + 1024, st,
-                            maps, a, m_pairs, items);
+                            maps, a, m_pairs, items, tile);
 }
-// Whether a request runs on CTA pairs: PAIR_RULE
-bool linear_on_pairs(const m26b_linear* L, bool bf16, uint32_t rows) {
-    const uint64_t items = uint64_t(L->tiles / 2) * ((rows + kLpTokens - 1) / kLpTokens);
-    if (rows <= 128 || items * 4 < uint64_t(L->sms)) return false;
+// Whether a request's activations (rows on vector boundaries) are converted inside the product's kernel. Up to 32 tokens (64 that
+// arrive quantised) that hides behind the weights; up to 128 it pays while a CTA has few chunks, since every weight tile repeats
+// it. Measured, inside / staged: 4,096 x 4,096 BF16 32 tokens 8.2 / 9.6 us, 64 10.9 / 8.7, E4M3 64 7.5 / 8.0, 128 11.3 / 10.3;
+// 1,000 x 1,024 (two chunks per CTA) BF16 40 tokens 5.2 / 5.6, 128 8.6 / 8.5, each with one launch less.
+bool linear_direct(const m26b_linear* L, bool bf16, uint32_t rows) {
+    if (rows <= (bf16 ? 32u : 64u)) return true;
+    if (rows > 128) return false;
+    const uint32_t chunks = L->k_pad / kChunkK, per_cta = chunks >> linear_log_split(L->tiles, uint64_t(L->sms), chunks);
+    return per_cta * rows <= (bf16 ? 256u : 512u);
+}
+// Token tile of the CTA-pair kernel for a request, or 0 if single CTAs (which can split K) finish it sooner, by cycles: rounds of
+// items over the GPU x cycles per item. A 128-wide chunk costs a pair 4 x pieces MMAs, each the slower of its math (tile / 2
+// cycles) and of shared memory at 128 B/clk (weight rows 32 cycles, token rows tile / 8, its share of filling the stage); a
+// single CTA of 128 tokens 768 (two pieces) or 512 cycles, shared memory again. The constants are what start, end and
+// hand-over of an item cost. A tile narrower than 256 tokens has to win by a tenth: it is more work in all, and the GPU is at
+// its power limit. Measured (4,096 x 4,096, pairs / single CTAs): 512 tokens 22.1 / 20.3 us, 768 26.6 / 31.1, E4M3 512 17.9 / 15.0,
+// 1,024 21.5 / 28.9; 1,536 tokens with tiles of 176 / 256: 46.0 / 53.1 us.
+uint32_t linear_pair_tile(const m26b_linear* L, bool bf16, uint32_t rows) {
+    if (rows <= 128) return 0;
     const int ctas = L->gated ? (bf16 ? linear_pair_ctas<2, true>(L) : linear_pair_ctas<1, true>(L)) : (bf16 ? linear_pair_ctas<2, false>(L) : linear_pair_ctas<1, false>(L));
-    return ctas > 0;
+    if (ctas < 2) return 0;
+    const uint64_t pairs = uint64_t(ctas) / 2, m_pairs = L->tiles / 2, chunks = L->k_pad / kChunkK, pieces = bf16 ? 2 : 1;
+    const auto pair_cost = [&](uint32_t tile) {
+        const uint64_t rounds = (m_pairs * ((rows + tile - 1) / tile) + pairs - 1) / pairs;
+        const uint64_t math = tile / 2, feed = 32 + tile / 8 + (128 + pieces * tile / 2) / (4 * pieces);
+        return rounds * (chunks * 4 * pieces * (math > feed ? math : feed) + 2000) + 10000;
+    };
+    uint32_t best = kLpTokens;
+    uint64_t cost = pair_cost(kLpTokens) * 9 / 10;
+    for (uint32_t tile = kLpTokens - 16; tile >= 64; tile -= 16)
+        if (pair_cost(tile) < cost) { best = tile; cost = pair_cost(tile); }
+    const uint64_t single = uint64_t(L->tiles) * ((rows + 127) / 128), sms = uint64_t(L->sms);
+    const uint32_t log_split = linear_log_split(single, sms, uint32_t(chunks));
+    const uint64_t single_cost = ((single << log_split) + sms - 1) / sms * ((chunks >> log_split) * (bf16 ? 768 : 512) + 4000);
+    return pair_cost(best) < single_cost ? best : 0;
 }
 
 // One pass of at most kLinearPassRows tokens.
@@ -144,10 +176,14 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
     const LinearArgs a{L->sf, sf, rows, rows_cap, L->n, L->k_pad / kChunkK, y, y_f32, y_pitch, fault, x, x_scales, x_pitch, L->k};
     TokenMaps mx{};
     cudaError_t e;
-    if (rows <= kLinearDirectRows && vec) {
-        e = rows <= 16 ? launch_linear_tile<16, true>(L, bf16, mx, a, st) : launch_linear_tile<32, true>(L, bf16, mx, a, st);
+    if (vec && linear_direct(L, bf16, rows)) {
+        if (rows <= 16) e = launch_linear_tile<16, true>(L, bf16, mx, a, st);
+        else if (rows <= 32) e = launch_linear_tile<32, true>(L, bf16, mx, a, st);
+        else if (rows <= 64) e = launch_linear_tile<64, true>(L, bf16, mx, a, st);
+        else e = launch_linear_tile<128, true>(L, bf16, mx, a, st);
     } else {
-        const SplitArgs sp{x, x_scales, x_pitch, vec, rows, L->k, L->k_pad, rows_cap, rows <= 64 ? 64u : 128u, ws, sf};
+        const uint32_t pair_tile = linear_pair_tile(L, bf16, rows), tile = pair_tile ? pair_tile : rows <= 64 ? 64u : 128u;
+        const SplitArgs sp{x, x_scales, x_pitch, vec, rows, L->k, L->k_pad, rows_cap, tile, rows <= 64 ? 1u : 0u, ws, sf};
         const uint64_t threads = uint64_t(rows) * (L->k_pad / 8);
         const unsigned blocks = unsigned((threads + 255) / 256);
         e = bf16 ? launch_dependent(linear_split_kernel<2>, blocks, 256, 0, st, sp) : launch_dependent(linear_split_kernel<1>, blocks, 256, 0, st, sp);
@@ -159,13 +195,14 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
             return true;
         };
         bool maps_ok;
-        if (linear_on_pairs(L, bf16, rows)) {
+        if (pair_tile) {
             LinearPairMaps pm{};
             pm.w = L->map_w; pm.sfa = L->map_sf;
-            maps_ok = boxes(pm.tok, 5) && make_sf_map(&pm.sfb, sf, uint64_t((rows + 127) / 128) * a.chunks * pieces, pieces);
+            const uint32_t blocks = (tile > 128 ? 2 : 1) * pieces;
+            maps_ok = boxes(pm.tok, 5) && make_sf_map(&pm.sfb, sf, uint64_t((rows + tile - 1) / tile) * a.chunks * blocks, blocks);
             if (maps_ok) {
-                if (L->gated) e = bf16 ? launch_linear_pair<2, true>(L, pm, a, st) : launch_linear_pair<1, true>(L, pm, a, st);
-                else e = bf16 ? launch_linear_pair<2, false>(L, pm, a, st) : launch_linear_pair<1, false>(L, pm, a, st);
+                if (L->gated) e = bf16 ? launch_linear_pair<2, true>(L, pm, a, tile, st) : launch_linear_pair<1, true>(L, pm, a, tile, st);
+                else e = bf16 ? launch_linear_pair<2, false>(L, pm, a, tile, st) : launch_linear_pair<1, false>(L, pm, a, tile, st);
             }
         } else {
             maps_ok = boxes(mx.box, 4);
@@ -269,7 +306,8 @@ void m26b_linear_free(m26b_linear* l) {
 uint64_t m26b_linear_workspace_bytes(const m26b_linear* l, uint32_t rows) {
     if (!l || !rows) return 0;
     const uint64_t cap = linear_rows_cap(rows);
-    return 2 * (cap * l->k_pad + (cap + 127) / 128 * (l->k_pad / kChunkK) * kScaleBlockBytes);
+    // two pieces of codes, and scale blocks: two per 128-token run, of which a tile of 64..256 tokens has at most (rows / 64 + 1)
+    return 2 * (cap * l->k_pad + (cap / 64 + 1) * (l->k_pad / kChunkK) * kScaleBlockBytes);
 }
 int m26b_linear_dev(const m26b_linear* l, const m26b_linear_args* args, void* stream, char* err, size_t errlen) {
     if (!l || !args || !(args->x_dtype == 0 || args->x_dtype == 2) || args->y_dtype < 0 || args->y_dtype > 1 || args->reserved) {

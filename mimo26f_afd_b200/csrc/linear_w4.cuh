@@ -121,9 +121,11 @@ struct SplitArgs {
     uint64_t pitch;              // elements
     int vec;                     // rows start on 16-byte (BF16) / 8-byte (E4M3) boundaries
     uint32_t rows, k, k_pad, rows_cap;
-    uint32_t lo_row;             // scale-block row of the second piece's first token: 64 (one block per chunk) or 128 (two)
+    // Scale blocks: [token tile of `tile` tokens][chunk][128-token run of the tile][piece][512]; with `joint` (tiles of 64) one block holds both
+    // pieces, the second's tokens from row 64 on.
+    uint32_t tile, joint;
     uint8_t* q;                  // [PIECES][rows_cap][k_pad]
-    uint8_t* sf;                 // [128-token tile][chunk][blocks][512]
+    uint8_t* sf;
 };
 // Four threads per K32 block, eight elements each.
 template <int PIECES>
@@ -172,12 +174,12 @@ __global__ void __launch_bounds__(256) linear_split_kernel(const SplitArgs p) {
     *reinterpret_cast<uint2*>(q) = hi;
     if constexpr (PIECES == 2) *reinterpret_cast<uint2*>(q + uint64_t(p.rows_cap) * p.k_pad) = lo;
     if ((g & 3u) == 0) {
-        const uint32_t blocks = PIECES == 2 && p.lo_row == 128 ? 2 : 1, r = row & 127u;
-        uint8_t* sf = p.sf + (uint64_t(row >> 7) * (p.k_pad / kChunkK) + (kb >> 2)) * blocks * kScaleBlockBytes;
-        sf[scale_block_offset(int(r), int(kb & 3u))] = uint8_t(scale);
+        const uint32_t t = row / p.tile, r = row % p.tile, blocks = p.joint ? 1 : (p.tile + 127) / 128 * PIECES;
+        uint8_t* sf = p.sf + (uint64_t(t) * (p.k_pad / kChunkK) + (kb >> 2)) * blocks * kScaleBlockBytes + (r >> 7) * PIECES * kScaleBlockBytes;
+        sf[scale_block_offset(int(r & 127u), int(kb & 3u))] = uint8_t(scale);
         if constexpr (PIECES == 2) {
-            const uint32_t lr = p.lo_row + r;
-            sf[(lr >> 7) * kScaleBlockBytes + scale_block_offset(int(lr & 127u), int(kb & 3u))] = uint8_t(scale - 4u);
+            if (p.joint) sf[scale_block_offset(int(64 + r), int(kb & 3u))] = uint8_t(scale - 4u);
+            else sf[kScaleBlockBytes + scale_block_offset(int(r & 127u), int(kb & 3u))] = uint8_t(scale - 4u);
         }
     }
 }
@@ -241,6 +243,8 @@ template <int B_ROWS, int PIECES>
 struct LinearTile {
     static constexpr int kN = PIECES * B_ROWS, kSfb = kN > 128 ? 2 : 1;    // operand rows, scale blocks of a chunk
     static constexpr int kCtasPerSm = B_ROWS <= 32 ? 2 : 1;
+    // epilogue warps, two or four per tensor-memory lane quadrant, and the converters of DIRECT kernels; a producer and an MMA warp in front
+    static constexpr int kConvWarps = B_ROWS <= 32 ? 8 : 16, kThreads = 64 + 32 * kConvWarps;
     static constexpr int kStageBytes = kTileM * 128 + kN * 128 + (1 + kSfb) * kScaleBlockBytes;
     static constexpr int kRedBytes = B_ROWS * kTileM * 4;                  // partial sums of a split K, and the gate / up exchange
     static constexpr int kFit = ((kCtasPerSm == 2 ? 111 : 224) * 1024 - kRedBytes) / kStageBytes;
@@ -259,9 +263,6 @@ struct LinearSmem {
     uint64_t full[T::kStages], empty[T::kStages], acc_full;
     uint32_t tmem_base, abort_flag;
 };
-constexpr int kConvWarps = 8;                    // epilogue warps: two per tensor-memory lane quadrant; the converters of DIRECT kernels
-constexpr int kLinearThreads = 64 + 32 * kConvWarps;     // a producer warp and an MMA warp in front
-
 // Eight activations of one row as they lie in memory, and their block's scale byte if they have one. The address is valid
 // whatever the place (rows and columns beyond the request read its last row and first columns and are dropped when the values
 // are used): with no branch around them, the loads of a whole chunk stay in flight.
@@ -293,6 +294,7 @@ struct RawX {
 template <int B_ROWS, int PIECES>
 struct LinearConverter {
     static constexpr uint32_t kStages = LinearTile<B_ROWS, PIECES>::kStages, kParts = B_ROWS / 8;       // kParts warps share a chunk
+    static constexpr uint32_t kConvWarps = LinearTile<B_ROWS, PIECES>::kConvWarps;
     // No more chunks at work than there are stages: a warp that has finished chunk i knows chunks up to i - kStages to be consumed,
     // so with a step of at most kStages the parity it waits for next cannot be that of a stage's use before last.
     static constexpr uint32_t kLanes = kConvWarps / kParts < kStages ? kConvWarps / kParts : kStages;
@@ -341,7 +343,7 @@ struct LinearConverter {
                 if constexpr (PIECES == 2) *reinterpret_cast<uint2*>(at + B_ROWS * 128) = lo[v];
                 if ((g & 3u) == 0) {
                     s.sfb[stage][scale_block_offset(int(r), int(g >> 2))] = uint8_t(scale[v]);
-                    if constexpr (PIECES == 2) s.sfb[stage][scale_block_offset(int(B_ROWS + r), int(g >> 2))] = uint8_t(scale[v] - 4u);
+                    if constexpr (PIECES == 2) s.sfb[stage][((B_ROWS + r) >> 7) * kScaleBlockBytes + scale_block_offset(int((B_ROWS + r) & 127u), int(g >> 2))] = uint8_t(scale[v] - 4u);
                 }
             }
             fence_async_smem();
@@ -357,13 +359,12 @@ struct LinearConverter {
 // finishing an equal part of the tile's features, so the result does not depend on timing. Token tiles start on multiples of 128
 // (their scale blocks hold 128 tokens): smaller B_ROWS serve requests of at most B_ROWS tokens.
 //
-// DIRECT (a few tokens): the epilogue warps, idle while the weights stream, turn the activations of each chunk into the
-// pieces in shared memory themselves; no second launch, no workspace. Every weight tile repeats that work, so larger requests
-// stage the pieces once (linear_split_kernel) and fetch them with TMA.
+// DIRECT (up to 128 tokens, rows on 16-byte boundaries): the epilogue warps, idle while the weights stream, turn the activations of
+// each chunk into the pieces in shared memory themselves; no second launch, no workspace. Every weight tile repeats that work, so
+// larger requests stage the pieces once (linear_split_kernel) and fetch them with TMA.
 template <int B_ROWS, int PIECES, bool GATED, bool DIRECT>
-__global__ void __launch_bounds__(kLinearThreads, (LinearTile<B_ROWS, PIECES>::kCtasPerSm))
+__global__ void __launch_bounds__((LinearTile<B_ROWS, PIECES>::kThreads), (LinearTile<B_ROWS, PIECES>::kCtasPerSm))
 linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps maps_x, const LinearArgs p, const uint32_t log_split) {
-    static_assert(!DIRECT || B_ROWS * PIECES <= 128, "one scale block per chunk");
     using T = LinearTile<B_ROWS, PIECES>;
     using Smem = LinearSmem<B_ROWS, PIECES>;
     extern __shared__ uint8_t smem_raw[];
@@ -444,7 +445,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         tmem_alloc(&s.tmem_base, T::kCols);      // while the first loads are under way; the epilogue warps learn the address below
         tmem_relinquish();
         tc_fence_before();
-        named_bar_sync(1, 32 + 32 * kConvWarps);
+        named_bar_sync(1, 32 + 32 * T::kConvWarps);
         tc_fence_after();
         const uint32_t tb = s.tmem_base;
         if (elect_one()) {
@@ -473,7 +474,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         __syncwarp();
         if (split > 1) cluster_wait();
     } else {
-        named_bar_sync(1, 32 + 32 * kConvWarps);
+        named_bar_sync(1, 32 + 32 * T::kConvWarps);
         tc_fence_after();
         const uint32_t tb = s.tmem_base;
         if constexpr (DIRECT) {
@@ -482,7 +483,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             conv.run(p, s, uint32_t(lane));
         }
         // ------------------------------------------------------------ epilogue, first half: tensor memory -> where it is added
-        const uint32_t q = uint32_t(warp) & 3u;            // lane quadrant; the quadrant's two warps take every other sixteen tokens
+        const uint32_t q = uint32_t(warp) & 3u;            // lane quadrant; the quadrant's warps take sixteen tokens in turn
         const uint32_t row = q * 32u + lane;               // weight row of the tile
         const bool ok = mbar_wait(&s.acc_full, 0, abort_flag);
         __syncwarp();
@@ -495,7 +496,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             const uint32_t owner = f >> log_run, slot = (f & ((1u << log_run) - 1)) + (GATED ? uint32_t(lane >> 4) << log_run : 0);
             const uint32_t base = (split > 1 ? cluster_map(smem_u32(s.red), owner) : smem_u32(s.red)) + slot * 4;
             const uint32_t feat = tile * (GATED ? 64 : kTileM) + f;
-            for (uint32_t col = uint32_t(warp - 2) / 4 * 16; col < n_mma; col += 32) {
+            for (uint32_t col = uint32_t(warp - 2) / 4 * 16; col < n_mma; col += T::kConvWarps * 4) {
                 uint32_t r[16];
                 tmem_ld16(t_acc + col, r);
                 if constexpr (PIECES == 2) {
@@ -524,7 +525,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         // -------------------------------------------------------- epilogue, second half: partial sums in rank order
         const uint32_t log_feats = (GATED ? 6 : 7) - log_split, feats = 1u << log_feats;
         const uint32_t feat0 = tile * (GATED ? 64 : kTileM) + rank * feats;
-        for (uint32_t i = threadIdx.x; i < n_valid << log_feats; i += kLinearThreads) {
+        for (uint32_t i = threadIdx.x; i < n_valid << log_feats; i += T::kThreads) {
             const uint32_t f = i & (feats - 1), col = i >> log_feats;
             if (feat0 + f >= p.n) continue;
             const float* from = s.red + (col << (7 - log_split)) + f;
@@ -540,14 +541,14 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 }
 
 // ---- the product on CTA pairs (prefill) -----------------------------------------------------------------------------
-// cta_group::2: two CTAs of a cluster run one MMA of M = 256 (128 weight rows each) x N = up to 256 tokens, half of the token rows in
-// each CTA's shared memory. What bounds a block-scaled MMA at prefill is shared memory, which feeds the operands (128 B/clk) and
+// cta_group::2: two CTAs of a cluster run one MMA of M = 256 (128 weight rows each) x N = `tile` tokens (at most 256), half of the token
+// rows in each CTA's shared memory. What bounds a block-scaled MMA at prefill is shared memory, which feeds the operands (128 B/clk) and
 // takes the loads: per 128-wide chunk and CTA this shape reads PIECES x 32 KB and fills 16 + PIECES x 16 KB in PIECES x 512 cycles of
 // math, 112 B/clk with two pieces; 128 tokens wide it would be 144, a single CTA of 128 x 128 tokens 192. The pieces
 // accumulate one after the other into the same 256 columns, which leaves the other half of tensor memory to the scales.
 // The accumulators are pulled into registers (64 per thread) and handed back before the epilogue's math, so that the next
 // item's MMAs run meanwhile. Barriers as in gemm_mx_pair.cuh: loads of both CTAs report to the first CTA's `full`.
-constexpr uint32_t kLpTokens = 256;
+constexpr uint32_t kLpTokens = 256;                        // widest token tile
 constexpr int kLpEpiWarps = 16, kLpThreads = 64 + 32 * kLpEpiWarps;
 constexpr uint32_t kLpSfSlots = 8, kLpSfStride = 32;       // scale slots above the accumulators: 4 columns of weights, 8 per piece of tokens
 
@@ -555,7 +556,7 @@ struct LinearPairMaps {
     CUtensorMap w;          // weight rows, box 128
     CUtensorMap tok[5];     // token rows, boxes of 128 / 64 / 32 / 16 / 8
     CUtensorMap sfa;        // weight scale blocks as rows of 128 u32, box 1
-    CUtensorMap sfb;        // token scale blocks, box PIECES
+    CUtensorMap sfb;        // token scale blocks, box: those of a tile's chunk
 };
 template <int PIECES>
 struct LinearPairSmem {
@@ -563,16 +564,16 @@ struct LinearPairSmem {
     alignas(1024) uint8_t a[kStages][kTileM * 128];
     alignas(1024) uint8_t b[kStages][PIECES * (kLpTokens / 2) * 128];
     alignas(128) uint8_t sfa[kStages][kScaleBlockBytes];
-    alignas(128) uint8_t sfb[kStages][2 * PIECES * kScaleBlockBytes];       // [128-token half of the tile][piece]
+    alignas(128) uint8_t sfb[kStages][2 * PIECES * kScaleBlockBytes];       // [128-token run of the tile][piece]
     uint64_t full[kStages], empty[kStages], acc_full, acc_empty;
     uint32_t tmem_base, abort_flag;
 };
 static_assert(sizeof(LinearPairSmem<2>) + 1024 <= 232448 && sizeof(LinearPairSmem<1>) + 1024 <= 232448, "a CTA has at most 227 KB of shared memory");
 
-// Items: 256 image rows x 256 tokens, the weight rows running fastest, strided over the pairs of the grid.
+// Items: 256 image rows x `tile` tokens, the weight rows running fastest, strided over the pairs of the grid.
 template <int PIECES, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
-linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs p, const uint32_t m_pairs, const uint32_t n_items) {
+linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs p, const uint32_t m_pairs, const uint32_t n_items, const uint32_t tile_n) {
     using Smem = LinearPairSmem<PIECES>;
     constexpr uint32_t kStages = Smem::kStages;
     extern __shared__ uint8_t smem_raw[];
@@ -596,7 +597,8 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
     tc_fence_after();
     grid_dep_launch();
     const uint32_t tb = s.tmem_base;
-    const auto tile_tokens = [&](uint32_t t) { const uint32_t left = p.rows - t * kLpTokens; return left < kLpTokens ? left : kLpTokens; };
+    const auto tile_tokens = [&](uint32_t t) { const uint32_t left = p.rows - t * tile_n; return left < tile_n ? left : tile_n; };
+    const uint32_t runs = tile_n > 128 ? 2 : 1;          // 128-token runs of a tile, one scale block each per piece
 
     if (warp == 0) {
         // ------------------------------------------------------------ producer (both CTAs)
@@ -606,9 +608,9 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
             bool ok = true;
             for (uint32_t it = pair_id; it < n_items && ok; it += n_pairs) {
                 const uint32_t m = it % m_pairs, t = it / m_pairs;
-                const uint32_t n_mma = (tile_tokens(t) + 15) & ~15u, half = n_mma >> 1, sf_tiles = n_mma > 128 ? 2 : 1;
+                const uint32_t n_mma = (tile_tokens(t) + 15) & ~15u, half = n_mma >> 1;
                 const uint32_t tile = 2 * m + rank;
-                const uint32_t tx = kTileM * 64 + PIECES * half * 128 + kScaleBlockBytes + sf_tiles * PIECES * kScaleBlockBytes;
+                const uint32_t tx = kTileM * 64 + PIECES * half * 128 + kScaleBlockBytes + runs * PIECES * kScaleBlockBytes;
                 const auto weights = [&](uint32_t c, uint32_t st) {
                     const uint32_t bar = cluster_map(smem_u32(&s.full[st]), 0);
                     if (rank == 0) mbar_expect_tx(&s.full[st], 2 * tx);        // the bytes of both CTAs' loads
@@ -636,13 +638,12 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
                             const uint32_t box = 128u >> b;
                             if (half - r >= box) {
                                 tma_load_2d_pair(s.b[stage] + (piece * (kLpTokens / 2) + r) * 128, &maps.tok[b], int(c * kChunkK),
-                                                 int(piece * p.rows_cap + t * kLpTokens + rank * half + r), bar);
+                                                 int(piece * p.rows_cap + t * tile_n + rank * half + r), bar);
                                 r += box;
                             }
                         }
                     }
-                    for (uint32_t h = 0; h < sf_tiles; ++h)
-                        tma_load_2d_pair(s.sfb[stage] + h * PIECES * kScaleBlockBytes, &maps.sfb, 0, int(((2 * t + h) * p.chunks + c) * PIECES), bar);
+                    tma_load_2d_pair(s.sfb[stage], &maps.sfb, 0, int((t * p.chunks + c) * runs * PIECES), bar);
                     ++issued;
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
@@ -676,7 +677,7 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
 #pragma unroll
                     for (uint32_t piece = 0; piece < PIECES; ++piece) {
                         tc_cp_scales_pair(t_sf + 4 + 8 * piece, sfb_d + piece * (kScaleBlockBytes >> 4));
-                        if (n_mma > 128) tc_cp_scales_pair(t_sf + 8 + 8 * piece, sfb_d + (PIECES + piece) * (kScaleBlockBytes >> 4));
+                        if (runs == 2) tc_cp_scales_pair(t_sf + 8 + 8 * piece, sfb_d + (PIECES + piece) * (kScaleBlockBytes >> 4));
                     }
                     const uint64_t ad = a_desc0 + stage * (sizeof(s.a[0]) >> 4), bd = b_desc0 + stage * (sizeof(s.b[0]) >> 4);
 #pragma unroll
@@ -716,7 +717,7 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
             const uint32_t tile = 2 * m + rank, feat = GATED ? tile * 64 + q * 16 + (lane & 15) : tile * kTileM + q * 32 + lane;
 #pragma unroll
             for (uint32_t g = 0; g < 4; ++g)
-                if (col0 + 16 * g < n_valid) store_columns<GATED>(p, r[g], t * kLpTokens + col0 + 16 * g, t * kLpTokens + n_valid, feat, lane);
+                if (col0 + 16 * g < n_valid) store_columns<GATED>(p, r[g], t * tile_n + col0 + 16 * g, t * tile_n + n_valid, feat, lane);
         }
     }
     tc_fence_before();
