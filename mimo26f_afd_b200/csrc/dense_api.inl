@@ -15,6 +15,7 @@ struct m26b_linear {
 namespace {
 
 constexpr uint32_t kLinearMaxDim = 1u << 20;
+constexpr uint32_t kDenseMaxRows = 0x7fffffffu;
 constexpr uint32_t kLinearPassRows = 8192;      // tokens per pass: bounds the workspace at 2 x 8192 x k bytes
 
 int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool gated, uint32_t n, uint32_t k, m26b_linear** out, char* err,
@@ -166,6 +167,17 @@ uint32_t linear_pair_tile(const m26b_linear* L, bool bf16, uint32_t rows) {
     return pair_cost(best) < single_cost ? best : 0;
 }
 
+template <int PIECES, bool VEC>
+cudaError_t launch_split(const SplitArgs& a, cudaStream_t st) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((a.k_pad / kChunkK + 7) / 8, (a.rows + 7) / 8); cfg.blockDim = dim3(256); cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, linear_split_kernel<PIECES, VEC>, a);
+}
+
 // One pass of at most kLinearPassRows tokens.
 int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x_scales, uint64_t x_pitch, uint32_t rows, void* y, int y_f32,
                 uint64_t y_pitch, uint8_t* ws, uint32_t* fault, cudaStream_t st, char* err, size_t errlen) {
@@ -183,10 +195,9 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
         else e = launch_linear_tile<128, true>(L, bf16, mx, a, st);
     } else {
         const uint32_t pair_tile = linear_pair_tile(L, bf16, rows), tile = pair_tile ? pair_tile : rows <= 64 ? 64u : 128u;
-        const SplitArgs sp{x, x_scales, x_pitch, vec, rows, L->k, L->k_pad, rows_cap, tile, rows <= 64 ? 1u : 0u, ws, sf};
-        const uint64_t threads = uint64_t(rows) * (L->k_pad / 8);
-        const unsigned blocks = unsigned((threads + 255) / 256);
-        e = bf16 ? launch_dependent(linear_split_kernel<2>, blocks, 256, 0, st, sp) : launch_dependent(linear_split_kernel<1>, blocks, 256, 0, st, sp);
+        const SplitArgs sp{x, x_scales, x_pitch, rows, L->k, L->k_pad, rows_cap, tile, rows <= 64 ? 1u : 0u, ws, sf};
+        if (bf16) e = vec ? launch_split<2, true>(sp, st) : launch_split<2, false>(sp, st);
+        else e = vec ? launch_split<1, true>(sp, st) : launch_split<1, false>(sp, st);
         if (e != cudaSuccess) { cudaGetLastError(); set_err(err, errlen, "m26b linear stage launch", e); return 2; }
         const uint64_t map_rows = uint64_t(pieces) * rows_cap;
         const auto boxes = [&](CUtensorMap* to, int count) {            // the boxes a token tile of this request can use
@@ -319,8 +330,8 @@ int m26b_linear_dev(const m26b_linear* l, const m26b_linear_args* args, void* st
     if (!rows) return 0;
     const bool bf16 = in.x_dtype == 0;
     const uint64_t x_pitch = in.x_pitch ? in.x_pitch : l->k, y_pitch = in.y_pitch ? in.y_pitch : l->n;
-    if (!in.x || !in.y || !in.fault_dev || (!bf16 && !in.x_scales) || x_pitch < l->k || y_pitch < l->n) {
-        set_msg(err, errlen, "m26b linear: bad pointers/pitch");
+    if (rows > kDenseMaxRows || !in.x || !in.y || !in.fault_dev || (!bf16 && !in.x_scales) || x_pitch < l->k || y_pitch < l->n) {
+        set_msg(err, errlen, "m26b linear: bad pointers/pitch/rows");
         return 1;
     }
     if ((bf16 && reinterpret_cast<uintptr_t>(in.x) % 2) || reinterpret_cast<uintptr_t>(in.y) % (in.y_dtype ? 4 : 2)) {
@@ -342,7 +353,6 @@ int m26b_linear_dev(const m26b_linear* l, const m26b_linear_args* args, void* st
                                    x_pitch, m, static_cast<uint8_t*>(in.y) + r0 * y_row, in.y_dtype, y_pitch, static_cast<uint8_t*>(in.workspace),
                                    in.fault_dev, static_cast<cudaStream_t>(stream), err, errlen);
         if (rc) return rc;
-        if (rows - r0 <= kLinearPassRows) break;       // r0 must not pass 32 bits
     }
     return 0;
 }
@@ -355,7 +365,7 @@ int m26b_block_norm_dev(const m26b_block_norm_args* args, void* stream, char* er
     const auto bad = [](int t) { return t < 0 || t > 1; };
     if (n_planes < 0 || n_planes > 8 || bad(y_dtype) || bad(h_dtype) || bad(w_dtype) || bad(n_dtype) || gate_kind < 0 || gate_kind > 3 || in.reserved ||
         (gate_kind != 0) != (in.gate != nullptr) || (!n_planes && (in.post_w || in.gate || !in.residual)) || (!in.h_out && !in.n_out) ||
-        (!in.n_out && in.pre_w) || !width || width > kNormMaxWidth) {
+        (!in.n_out && in.pre_w) || !width || width > kNormMaxWidth || rows > kDenseMaxRows) {
         set_msg(err, errlen, "m26b block norm: bad arguments");
         return 1;
     }

@@ -119,7 +119,6 @@ struct SplitArgs {
     const void* x;
     const uint8_t* x_scales;     // PIECES 1: [rows][k / 32]
     uint64_t pitch;              // elements
-    int vec;                     // rows start on 16-byte (BF16) / 8-byte (E4M3) boundaries
     uint32_t rows, k, k_pad, rows_cap;
     // Scale blocks: [token tile of `tile` tokens][chunk][128-token run of the tile][piece][512]; with `joint` (tiles of 64) one block holds both
     // pieces, the second's tokens from row 64 on.
@@ -127,59 +126,79 @@ struct SplitArgs {
     uint8_t* q;                  // [PIECES][rows_cap][k_pad]
     uint8_t* sf;
 };
-// Four threads per K32 block, eight elements each.
-template <int PIECES>
+// A warp takes one 128-wide chunk of eight rows: sixteen lanes per row, eight elements each, two rows at a time; all its loads are
+// issued first. VEC: rows start on 16-byte (BF16) / 8-byte (E4M3) boundaries. What bounds it is HBM and L2: 8,192 x 4,096 BF16 reads 67 MB and
+// writes 67 MB of codes (a thread per eight elements, with the row and the tile found by division: 34 us).
+template <int PIECES, bool VEC>
 __global__ void __launch_bounds__(256) linear_split_kernel(const SplitArgs p) {
     grid_dep_wait();             // x, and the workspace that an earlier call may still read
     grid_dep_launch();
-    const uint32_t groups = p.k_pad / 8;
-    const uint64_t id = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    const uint64_t total = uint64_t(p.rows) * groups;      // a multiple of 16: the four threads of a block stay together
-    if (id >= total) return;
-    const uint32_t row = uint32_t(id / groups), g = uint32_t(id % groups), kb = g >> 2;
-    const uint64_t at = uint64_t(row) * p.pitch + uint64_t(g) * 8;
-    const bool real = g * 8 < p.k;
-    uint32_t scale = 127;
-    uint2 hi = make_uint2(0, 0), lo = make_uint2(0, 0);
-    if constexpr (PIECES == 2) {
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (real) {
+    const uint32_t lane = threadIdx.x & 31u, chunks = p.k_pad / kChunkK, c = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (c >= chunks) return;
+    const uint32_t g = lane & 15u, col = c * kChunkK + g * 8, row0 = blockIdx.y * 8;
+    const bool inside = col < p.k;
+    const uint32_t t = row0 / p.tile, r0 = row0 - t * p.tile;                  // eight rows never straddle a tile: tiles are multiples of 16
+    uint32_t w[4][PIECES == 2 ? 4 : 2], scale[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        uint32_t row = row0 + 2 * v + (lane >> 4);
+        row = row < p.rows ? row : p.rows - 1;                                 // beyond the request: read its last row, write nothing
+        const uint64_t at = uint64_t(row) * p.pitch + (inside ? col : 0);
+        if constexpr (PIECES == 2) {
             const uint16_t* x = static_cast<const uint16_t*>(p.x) + at;
-            if (p.vec) {
+            if constexpr (VEC) {
                 const uint4 a = *reinterpret_cast<const uint4*>(x);
-                w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+                w[v][0] = a.x; w[v][1] = a.y; w[v][2] = a.z; w[v][3] = a.w;
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = uint32_t(x[2 * e]) | uint32_t(x[2 * e + 1]) << 16;
+                for (int e = 0; e < 4; ++e) w[v][e] = uint32_t(x[2 * e]) | uint32_t(x[2 * e + 1]) << 16;
             }
-        }
-        const uint32_t amax = block_amax(w, 0xfu << (threadIdx.x & 28u));
-        const bool bad = amax >= 0x7f800000u;
-        if (!bad) scale = split_scale_byte(amax);
-        split8(w, scale, bad, hi, lo);
-    } else if (real) {
-        const uint8_t* x = static_cast<const uint8_t*>(p.x) + at;
-        if (p.vec) {
-            hi = *reinterpret_cast<const uint2*>(x);
+            scale[v] = 127;
         } else {
-            uint32_t o[2] = {0, 0};
+            const uint8_t* x = static_cast<const uint8_t*>(p.x) + at;
+            if constexpr (VEC) {
+                const uint2 a = *reinterpret_cast<const uint2*>(x);
+                w[v][0] = a.x; w[v][1] = a.y;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e >> 2] |= uint32_t(x[e]) << (8 * (e & 3));
-            hi = make_uint2(o[0], o[1]);
+                for (int e = 0; e < 2; ++e) w[v][e] = uint32_t(x[4 * e]) | uint32_t(x[4 * e + 1]) << 8 | uint32_t(x[4 * e + 2]) << 16 | uint32_t(x[4 * e + 3]) << 24;
+            }
+            scale[v] = p.x_scales[uint64_t(row) * (p.k / kBlockK) + (inside ? col : 0) / kBlockK];
         }
-        scale = p.x_scales[uint64_t(row) * (p.k / 32) + kb];
-        if (scale == 255u) { scale = 127; hi = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu); }      // a NaN scale
     }
-    uint8_t* q = p.q + uint64_t(row) * p.k_pad + uint64_t(g) * 8;
-    *reinterpret_cast<uint2*>(q) = hi;
-    if constexpr (PIECES == 2) *reinterpret_cast<uint2*>(q + uint64_t(p.rows_cap) * p.k_pad) = lo;
-    if ((g & 3u) == 0) {
-        const uint32_t t = row / p.tile, r = row % p.tile, blocks = p.joint ? 1 : (p.tile + 127) / 128 * PIECES;
-        uint8_t* sf = p.sf + (uint64_t(t) * (p.k_pad / kChunkK) + (kb >> 2)) * blocks * kScaleBlockBytes + (r >> 7) * PIECES * kScaleBlockBytes;
-        sf[scale_block_offset(int(r & 127u), int(kb & 3u))] = uint8_t(scale);
+    uint2 hi[4], lo[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+#pragma unroll
+        for (uint32_t& word : w[v]) word = inside ? word : 0u;
         if constexpr (PIECES == 2) {
-            if (p.joint) sf[scale_block_offset(int(64 + r), int(kb & 3u))] = uint8_t(scale - 4u);
-            else sf[kScaleBlockBytes + scale_block_offset(int(r & 127u), int(kb & 3u))] = uint8_t(scale - 4u);
+            const uint32_t amax = block_amax(w[v], 0xffffffffu);
+            const bool bad = amax >= 0x7f800000u;
+            scale[v] = bad ? 127u : split_scale_byte(amax);
+            split8(w[v], scale[v], bad, hi[v], lo[v]);
+        } else {
+            const bool nan = inside && scale[v] == 255u;                       // a NaN scale
+            scale[v] = nan || !inside ? 127u : scale[v];
+            hi[v] = nan ? make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu) : make_uint2(w[v][0], w[v][1]);
+        }
+    }
+    uint8_t* sf = p.sf + (uint64_t(t) * chunks + c) * (p.joint ? 1 : (p.tile + 127) / 128 * PIECES) * kScaleBlockBytes + (r0 >> 7) * PIECES * kScaleBlockBytes;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        const uint32_t own = lane & 16u, row = row0 + 2 * v + (own >> 4), r = (r0 & 127u) + 2 * v + (own >> 4);
+        uint32_t word = 0;                                                     // the row's four scale bytes of the chunk
+#pragma unroll
+        for (int b = 0; b < 4; ++b) word |= __shfl_sync(0xffffffffu, scale[v], own + 4 * b) << (8 * b);
+        if (row >= p.rows) continue;
+        uint8_t* q = p.q + uint64_t(row) * p.k_pad + col;
+        *reinterpret_cast<uint2*>(q) = hi[v];
+        if constexpr (PIECES == 2) *reinterpret_cast<uint2*>(q + uint64_t(p.rows_cap) * p.k_pad) = lo[v];
+        if (g == 0) {
+            *reinterpret_cast<uint32_t*>(sf + scale_block_offset(int(r), 0)) = word;
+            if constexpr (PIECES == 2) {                                       // every byte is at least 4
+                uint8_t* sl = p.joint ? sf + scale_block_offset(int(64 + r), 0) : sf + kScaleBlockBytes + scale_block_offset(int(r), 0);
+                *reinterpret_cast<uint32_t*>(sl) = word - 0x04040404u;
+            }
         }
     }
 }

@@ -27,7 +27,7 @@ def test_block_norm_without_rows_is_no_work():
     dict(planes=[], post_w=P), dict(planes=[], gate=P, gate_kind=1), dict(gate=P), dict(gate_kind=2), dict(gate=P, gate_kind=4),
     dict(gate=P, gate_kind=-1), dict(y_dtype=2), dict(h_dtype=-1), dict(n_dtype=2), dict(w_dtype=3), dict(h_out=None, n_out=None),
     dict(n_out=None, pre_w=P), dict(eps=0.0), dict(eps=-1e-6), dict(eps=float("nan")), dict(eps=float("inf")),
-    dict(y_pitch=63), dict(h_pitch=63), dict(n_pitch=1),
+    dict(rows=1 << 31), dict(y_pitch=63), dict(h_pitch=63), dict(n_pitch=1),
     dict(planes=[P + 1]), dict(planes=[P + 2], y_dtype=1), dict(residual=P + 2), dict(n_out=P + 1), dict(pre_w=P + 2),
     dict(gate=P + 2, gate_kind=1), dict(gate=P + 1, gate_kind=3),
 ])

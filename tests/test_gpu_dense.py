@@ -328,6 +328,90 @@ def test_pitches_and_alignment_and_what_lies_between_the_rows(torch, rows, x_off
         assert bool((yb == -77.0).all())                        # nothing outside the rows was written
 
 
+@pytest.mark.parametrize("rows", [3, 40, 150])
+@pytest.mark.parametrize("off,pad", [(0, 8), (1, 0), (4, 4), (8, 3)])
+def test_quantised_rows_of_any_alignment(torch, rows, off, pad):
+    import mimo26f_afd_b200 as M
+
+    n, k = 70, 160
+    g = gen(torch, rows + off)
+    w, s = make_weights(torch, n, k, g)
+    qb = torch.full((off + rows * (k + pad),), 0x7f, dtype=torch.uint8, device="cuda")
+    q = torch.as_strided(qb, (rows, k), (k + pad, 1), off)
+    q.copy_(torch.randint(0, 127, (rows, k), dtype=torch.uint8, device="cuda", generator=g))
+    xs = torch.randint(110, 130, (rows, k // 32), dtype=torch.uint8, device="cuda", generator=g)
+    y, bound = product_and_bound(torch, e4m3_f64(torch, q, xs), weight_f64(torch, w, s), quantised=True)
+    check(torch, Runner(torch, M.Linear.new(w, s, n, k), rows)(q, rows, x_scales=xs, x_pitch=k + pad), y, rounded(y, bound, False))
+
+
+def test_rows_more_than_four_gigabytes_apart(torch):
+    """Offsets past 32 bits, in bytes and in elements."""
+    import mimo26f_afd_b200 as M
+
+    n, k, pitch = 64, 64, (1 << 32) + 64
+    g = gen(torch, 17)
+    w, s = make_weights(torch, n, k, g)
+    xb, yb = (torch.empty(pitch + 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    x, y = (torch.as_strided(b, (2, 64), (pitch, 1)) for b in (xb, yb))
+    x.copy_(torch.randn(2, k, device="cuda", generator=g))
+    want, bound = product_and_bound(torch, x.double(), weight_f64(torch, w, s))
+    run = Runner(torch, M.Linear.new(w, s, n, k), 2)
+    check(torch, run(x, 2, x_pitch=pitch, y=y, y_pitch=pitch, f32=False), want, rounded(want, bound, True))
+    for width in (64, 63, 61):                                    # rows in vectors of eight, of four, and element by element
+        off = 1 if width == 61 else 0
+        xv, out = (torch.as_strided(b, (2, width), (pitch, 1), off) for b in (xb, yb))
+        out.zero_()
+        M.block_norm_dev([xv], None, 2, width, y_pitch=pitch, n_out=out, n_pitch=pitch)
+        torch.cuda.synchronize()
+        _, want = norm_f64([xv], None, None, None, 0, None, 1e-6, 1.0, 1.0)
+        assert bool(((out.double() - want).abs() <= (2.0**-8 + 64 * U) * want.abs()).all())
+
+
+def test_first_calls_inside_a_capture(torch):
+    """A fresh process whose first call of every variant is captured (nothing may need a call outside before), then replayed."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+
+    code = """
+import sys; sys.path.insert(0, %r)
+import torch, mimo26f_afd_b200 as M
+def mk(n, k):
+    return torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device='cuda'), torch.full((n, k // 32), 120, dtype=torch.uint8, device='cuda')
+n, k = 9600, 256
+w, s = mk(n, k)
+lin, gat = M.Linear.new(w, s, n, k), M.Linear.gated(w, s, w, s, n, k)
+fault = torch.zeros(1, dtype=torch.int32, device='cuda')
+ws = torch.empty(lin.workspace_bytes(600), dtype=torch.uint8, device='cuda')
+jobs = []
+for rows in (1, 20, 50, 100, 600):
+    x = torch.randn(rows, k, device='cuda').bfloat16()
+    jobs.append((x, torch.zeros(rows, n, device='cuda'), torch.zeros(rows, n, device='cuda'), torch.zeros(rows, k, device='cuda'), torch.zeros(rows, k - 1, device='cuda')))
+torch.cuda.synchronize()
+def run(st):
+    for x, a, b, h, h1 in jobs:
+        r = x.shape[0]
+        M.linear_dev(lin, x, r, a, y_dtype=1, workspace=ws, fault=fault, stream=st)
+        M.linear_dev(gat, x, r, b, y_dtype=1, workspace=ws, fault=fault, stream=st)
+        M.block_norm_dev([x], None, r, k, n_out=h, n_dtype=1, stream=st)
+        M.block_norm_dev([x], None, r, k - 1, n_out=h1, n_dtype=1, stream=st)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    run(torch.cuda.current_stream().cuda_stream)
+g.replay(); torch.cuda.synchronize()
+got = [[t.clone() for t in j[1:]] for j in jobs]
+for j in jobs:
+    for t in j[1:]: t.zero_()
+run(None); torch.cuda.synchronize()
+assert all(torch.equal(p, q) and float(p.abs().sum()) > 0 for o, j in zip(got, jobs) for p, q in zip(o, j[1:]))
+assert int(fault) == 0
+print('captured')
+""" % ROOT
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 def test_weights_of_any_alignment(torch):
     import mimo26f_afd_b200 as M
 
