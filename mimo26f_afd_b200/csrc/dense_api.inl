@@ -167,15 +167,14 @@ uint32_t linear_pair_tile(const m26b_linear* L, bool bf16, uint32_t rows) {
     return pair_cost(best) < single_cost ? best : 0;
 }
 
-template <int PIECES, bool VEC>
-cudaError_t launch_split(const SplitArgs& a, cudaStream_t st) {
+cudaError_t launch_stage(void (*kernel)(SplitArgs), dim3 grid, const SplitArgs& a, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((a.k_pad / kChunkK + 7) / 8, (a.rows + 7) / 8); cfg.blockDim = dim3(256); cfg.stream = st;
+    cfg.gridDim = grid; cfg.blockDim = dim3(256); cfg.stream = st;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, linear_split_kernel<PIECES, VEC>, a);
+    return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 // One pass of at most kLinearPassRows tokens.
@@ -196,13 +195,20 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
     } else {
         const uint32_t pair_tile = linear_pair_tile(L, bf16, rows), tile = pair_tile ? pair_tile : rows <= 64 ? 64u : 128u;
         const SplitArgs sp{x, x_scales, x_pitch, rows, L->k, L->k_pad, rows_cap, tile, rows <= 64 ? 1u : 0u, ws, sf};
-        if (bf16) e = vec ? launch_split<2, true>(sp, st) : launch_split<2, false>(sp, st);
-        else e = vec ? launch_split<1, true>(sp, st) : launch_split<1, false>(sp, st);
+        // quantised rows on 16-byte boundaries are loaded from where they are
+        const bool in_place = !bf16 && xa % 16 == 0 && x_pitch % 16 == 0;
+        if (in_place) e = launch_stage(linear_scales_kernel, dim3((sp.k_pad / kChunkK + 31) / 32, (rows + 7) / 8), sp, st);
+        else {
+            const dim3 grid((sp.k_pad / kChunkK + 7) / 8, (rows + 7) / 8);
+            if (bf16) e = launch_stage(vec ? linear_split_kernel<2, true> : linear_split_kernel<2, false>, grid, sp, st);
+            else e = launch_stage(vec ? linear_split_kernel<1, true> : linear_split_kernel<1, false>, grid, sp, st);
+        }
         if (e != cudaSuccess) { cudaGetLastError(); set_err(err, errlen, "m26b linear stage launch", e); return 2; }
-        const uint64_t map_rows = uint64_t(pieces) * rows_cap;
+        const uint64_t map_rows = in_place ? rows : uint64_t(pieces) * rows_cap, map_cols = in_place ? L->k : L->k_pad, map_pitch = in_place ? x_pitch : L->k_pad;
+        void* map_base = in_place ? const_cast<void*>(x) : ws;
         const auto boxes = [&](CUtensorMap* to, int count) {            // the boxes a token tile of this request can use
             for (int i = 0; i < count; ++i)
-                if ((128u >> i) <= rows_cap && !make_map(&to[i], false, ws, L->k_pad, map_rows, L->k_pad, 128u >> i)) return false;
+                if ((128u >> i) <= rows_cap && !make_map(&to[i], false, map_base, map_cols, map_rows, map_pitch, 128u >> i)) return false;
             return true;
         };
         bool maps_ok;

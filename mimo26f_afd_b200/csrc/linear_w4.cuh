@@ -203,6 +203,22 @@ __global__ void __launch_bounds__(256) linear_split_kernel(const SplitArgs p) {
     }
 }
 
+// Quantised activations whose rows TMA can take where they are (16-byte boundaries): only their scale bytes are staged, one thread per
+// row and chunk. Byte 255 is a NaN to the MMA too.
+__global__ void __launch_bounds__(256) linear_scales_kernel(const SplitArgs p) {
+    grid_dep_wait();             // the scales, and the workspace that an earlier call may still read
+    grid_dep_launch();
+    const uint32_t chunks = p.k_pad / kChunkK, blocks = p.k / kBlockK, row = blockIdx.y * 8 + (threadIdx.x >> 5), c = blockIdx.x * 32 + (threadIdx.x & 31u);
+    if (row >= p.rows || c >= chunks) return;
+    const uint8_t* from = p.x_scales + uint64_t(row) * blocks;
+    uint32_t word = 0;
+#pragma unroll
+    for (uint32_t b = 0; b < 4; ++b) word |= (4 * c + b < blocks ? uint32_t(from[4 * c + b]) : 127u) << (8 * b);
+    const uint32_t t = row / p.tile, r = row - t * p.tile;
+    uint8_t* sf = p.sf + ((uint64_t(t) * chunks + c) * ((p.tile + 127) / 128) + (r >> 7)) * kScaleBlockBytes;
+    *reinterpret_cast<uint32_t*>(sf + scale_block_offset(int(r & 127u), 0)) = word;
+}
+
 // ---- the product ---------------------------------------------------------------------------------------------------
 struct LinearArgs {
     const uint8_t* sfa;          // weight scales

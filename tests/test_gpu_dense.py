@@ -117,7 +117,7 @@ def test_linear_extents(torch, n, k):
     check(torch, run(x, rows), y, rounded(y, bound, False))
 
 
-@pytest.mark.parametrize("rows", [1, 3, 8, 13, 16, 23, 32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 3, 8, 13, 16, 23, 32, 41, 64, 90, 120, 127, 128])
 @pytest.mark.parametrize("n", [9000, 30000])
 def test_many_weight_tiles_with_many_chunks_each(torch, rows, n):
     """Enough tiles that K is hardly split: every stage of the pipeline is reused several times in one CTA."""
@@ -272,18 +272,22 @@ def test_a_row_with_a_nonfinite_value_is_nan_and_the_others_are_untouched(torch,
 def test_quantised_rows_with_nan_codes_or_scales_are_nan(torch):
     import mimo26f_afd_b200 as M
 
-    n, k, rows = 128, 128, 6
+    n, k = 9728, 128
     g = gen(torch, 10)
     w, s = make_weights(torch, n, k, g)
-    q = torch.full((rows, k), 0x38, dtype=torch.uint8, device="cuda")
-    xs = torch.full((rows, k // 32), 127, dtype=torch.uint8, device="cuda")
-    q[1, 40] = 0x7f
-    q[2, 127] = 0xff
-    xs[4, 3] = 255
-    y = Runner(torch, M.Linear.new(w, s, n, k), rows)(q, rows, x_scales=xs)
-    torch.cuda.synchronize()
-    nan = torch.isnan(y)
-    assert nan.all(1).tolist() == [False, True, True, False, True, False] and nan.any(1).tolist() == nan.all(1).tolist()
+    layer = M.Linear.new(w, s, n, k)
+    for rows in (6, 70, 500):                                   # converted in the kernel, staged, on CTA pairs
+        for pitch in (k, k + 8):                                # rows TMA can take in place, and not
+            q = torch.full((rows, pitch), 0x38, dtype=torch.uint8, device="cuda")[:, :k]
+            xs = torch.full((rows, k // 32), 127, dtype=torch.uint8, device="cuda")
+            q[1, 40] = 0x7f
+            q[2, 127] = 0xff
+            xs[4, 3] = 255
+            y = Runner(torch, layer, rows)(q, rows, x_scales=xs, x_pitch=pitch)
+            torch.cuda.synchronize()
+            nan = torch.isnan(y)
+            want = [i in (1, 2, 4) for i in range(rows)]
+            assert nan.all(1).tolist() == want and nan.any(1).tolist() == want
 
 
 def test_scale_bytes_at_the_ends_of_their_range(torch):
@@ -329,7 +333,7 @@ def test_pitches_and_alignment_and_what_lies_between_the_rows(torch, rows, x_off
 
 
 @pytest.mark.parametrize("rows", [3, 40, 150])
-@pytest.mark.parametrize("off,pad", [(0, 8), (1, 0), (4, 4), (8, 3)])
+@pytest.mark.parametrize("off,pad", [(0, 0), (0, 16), (0, 8), (1, 0), (4, 4), (8, 3), (16, 32)])
 def test_quantised_rows_of_any_alignment(torch, rows, off, pad):
     import mimo26f_afd_b200 as M
 
@@ -673,6 +677,66 @@ def test_norm_of_zero_huge_and_nonfinite_rows(torch):
 
 
 # ----------------------------------------------------------------------------------------------------------- together
+def test_a_moe_block_with_a_shared_expert_between_two_norms(torch):
+    """norm -> routed experts (m26b_ffn_dev) and a shared expert (gated, linear) -> their sum, the residual and the next norm, on one
+    stream and replayed from a graph; the sum is m26b_rank_sum_residual_dev's bits, the shared expert is held to 64 bits."""
+    import mimo26f_afd_b200 as M
+    from mimo26f_afd_b200 import synth
+
+    rows, H, I = 16, 4096, 2048
+    dev = torch.device("cuda:0")
+    g = gen(torch, 4)
+    routed_w = synth.layer_torch(7, dev)
+    layer = M.Layer.from_checkpoint(*[routed_w[n] for n in synth.TENSORS])
+    shared = {n: routed_w[n][5] for n in synth.TENSORS}          # expert 5's tensors stand for the shared expert's
+    up = M.Linear.gated(shared["gate_w"], shared["gate_s"], shared["up_w"], shared["up_s"], I, H)
+    down = M.Linear.new(shared["down_w"], shared["down_s"], H, I)
+    scratch = M.Scratch()
+    ids, wts = (torch.from_numpy(np.ascontiguousarray(a)).cuda() for a in synth.routing(7, rows, 0.0))
+    ws = torch.empty(max(up.workspace_bytes(rows), down.workspace_bytes(rows)), dtype=torch.uint8, device="cuda")
+    fault = torch.zeros(1, dtype=torch.int32, device="cuda")
+    h0 = torch.randn(rows, H, device="cuda", generator=g)
+    w1, w2 = (1 + 0.1 * torch.randn(H, device="cuda", generator=g) for _ in range(2))
+    h = torch.zeros_like(h0)
+    n1, routed, y, n2 = (torch.zeros(rows, H, dtype=torch.bfloat16, device="cuda") for _ in range(4))
+    a = torch.zeros(rows, I, dtype=torch.bfloat16, device="cuda")
+
+    def step(st):
+        M.block_norm_dev([], h0, rows, H, pre_w=w1, n_out=n1, stream=st)
+        M.ffn_dev(layer, scratch, n1, ids, wts, rows, routed, stream=st)
+        M.linear_dev(up, n1, rows, a, workspace=ws, fault=fault, stream=st)
+        M.linear_dev(down, a, rows, y, workspace=ws, fault=fault, stream=st)
+        M.block_norm_dev([routed, y], h0, rows, H, pre_w=w2, h_out=h, n_out=n2, stream=st)
+
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    step(side.cuda_stream)
+    scratch.status(side.cuda_stream)
+    torch.cuda.synchronize()
+    first = [t.clone() for t in (n1, routed, a, y, h, n2)]
+    want = torch.empty_like(h0)
+    M.rank_sum_dev([routed, y], rows * H, want, residual=h0)
+    torch.cuda.synchronize()
+    assert torch.equal(h, want)
+    _, nn = norm_f64([], h, None, None, 0, w2, 1e-6, 1.0, 1.0)
+    assert bool(((n2.double() - nn).abs() <= (2.0**-8 + 64 * U) * nn.abs()).all())
+    G, Up, D = (weight_f64(torch, shared[p + "_w"], shared[p + "_s"]) for p in ("gate", "up", "down"))
+    p, dp = product_and_bound(torch, n1.double(), G)
+    q, dq = product_and_bound(torch, n1.double(), Up)
+    silu = p * torch.sigmoid(p)
+    check(torch, a, silu * q, rounded(silu * q, 1.1 * dp * (q.abs() + dq) + silu.abs() * dq + 2.0**-19 * (silu * q).abs(), True))
+    z, dz = product_and_bound(torch, a.double(), D)
+    check(torch, y, z, rounded(z, dz, True))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(side.cuda_stream)
+    for t in (n1, routed, a, y, h, n2):
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(first, (n1, routed, a, y, h, n2))) and int(fault) == 0
+
+
 @pytest.mark.parametrize("rows", [1, 16, 140])
 def test_a_dense_block_between_two_norms(torch, rows):
     """norm -> gated -> linear -> norm, as a dense block of a decoder runs them: captured once and replayed, against 64 bits
