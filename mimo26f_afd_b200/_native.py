@@ -72,8 +72,9 @@ def lib() -> C.CDLL:
     L.m26b_linear_free.restype = None
     L.m26b_linear_workspace_bytes.argtypes = [vp, C.c_uint32]
     L.m26b_linear_workspace_bytes.restype = C.c_uint64
-    L.m26b_linear_dev.argtypes = [vp, C.c_char_p, vp, *err]       # the argument record as packed bytes (dense.py)
-    L.m26b_block_norm_dev.argtypes = [C.c_char_p, vp, *err]     # the argument record as packed bytes (dense.py)
+    # the argument records as packed bytes and the error buffer as an address (dense.py): calls of a decode step, several per layer
+    L.m26b_linear_dev.argtypes = [vp, C.c_char_p, vp, vp, C.c_size_t]
+    L.m26b_block_norm_dev.argtypes = [C.c_char_p, vp, vp, C.c_size_t]
     L.m26b_quantize_dev.argtypes = [vp, C.c_int, C.c_uint64, C.c_int, u8p, u8p, u32p, vp, *err]
     L.m26b_route_reduce_dev.argtypes = [f32p, f32p, C.c_uint32, f32p, u16p, u32p, vp, *err]
     L.m26b_rank_sum_dev.argtypes = [C.POINTER(vp), C.c_int, C.c_uint64, f32p, vp, *err]

@@ -26,11 +26,13 @@ _local = threading.local()
 
 
 def _err():
-    """This thread's error buffer (a decode step makes several calls per layer; a fresh buffer each costs more than the check)."""
+    """This thread's error buffer and its address (a decode step makes several calls per layer; a fresh buffer each costs more
+    than the rest of the check)."""
     try:
         return _local.err
     except AttributeError:
-        _local.err = C.create_string_buffer(256)
+        buf = C.create_string_buffer(256)
+        _local.err = buf, C.addressof(buf)
         return _local.err
 
 
@@ -99,10 +101,10 @@ def linear_dev(layer: Linear, x, rows: int, y, *, x_dtype: int = X_BF16, x_scale
                                  x_dtype, y_dtype, 0)
     except (struct.error, OverflowError) as e:        # a negative or oversized number
         raise ExpertError(1, f"m26b linear: bad arguments ({e})") from None
-    err = _err()
-    rc = _native.lib().m26b_linear_dev(layer._h, args, _addr(stream), err, 256)
+    buf, at = _err()
+    rc = _native.lib().m26b_linear_dev(layer._h, args, _addr(stream), at, 256)
     if rc:
-        _check(rc, err)
+        _check(rc, buf)
 
 
 def block_norm_dev(planes, residual, rows: int, width: int, *, post_w=None, gate=None, gate_kind: int = GATE_NONE, y_dtype: int = 0,
@@ -115,15 +117,20 @@ def block_norm_dev(planes, residual, rows: int, width: int, *, post_w=None, gate
     if n > 8:
         raise ExpertError(1, "m26b block norm: bad arguments")
     try:
-        args = _NORM_ARGS.pack(*map(_addr, planes), *_PAD[n], _addr(post_w), _addr(gate), _addr(residual), _addr(pre_w), _addr(h_out),
-                               _addr(n_out), y_pitch, h_pitch, n_pitch, y_scale, residual_scale, eps, rows, width, n, gate_kind, y_dtype, h_dtype,
-                               n_dtype, w_dtype, 0)
+        if n == 1:
+            args = _NORM_ARGS.pack(_addr(planes[0]), 0, 0, 0, 0, 0, 0, 0, _addr(post_w), _addr(gate), _addr(residual), _addr(pre_w), _addr(h_out),
+                                   _addr(n_out), y_pitch, h_pitch, n_pitch, y_scale, residual_scale, eps, rows, width, 1, gate_kind, y_dtype,
+                                   h_dtype, n_dtype, w_dtype, 0)
+        else:
+            args = _NORM_ARGS.pack(*map(_addr, planes), *_PAD[n], _addr(post_w), _addr(gate), _addr(residual), _addr(pre_w), _addr(h_out),
+                                   _addr(n_out), y_pitch, h_pitch, n_pitch, y_scale, residual_scale, eps, rows, width, n, gate_kind, y_dtype,
+                                   h_dtype, n_dtype, w_dtype, 0)
     except (struct.error, OverflowError) as e:        # a negative or oversized number
         raise ExpertError(1, f"m26b block norm: bad arguments ({e})") from None
-    err = _err()
-    rc = _native.lib().m26b_block_norm_dev(args, _addr(stream), err, 256)
+    buf, at = _err()
+    rc = _native.lib().m26b_block_norm_dev(args, _addr(stream), at, 256)
     if rc:
-        _check(rc, err)
+        _check(rc, buf)
 
 
 _PAD = [(0,) * (8 - i) for i in range(9)]

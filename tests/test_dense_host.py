@@ -96,8 +96,9 @@ def test_linear_refuses_null_tensors_and_handles():
         assert e.value.code == 1
     lib = _native.lib()
     err = ctypes.create_string_buffer(256)
-    assert lib.m26b_linear_dev(None, b"\0" * 256, None, err, 256) == 1 and b"bad handle" in err.value
-    assert lib.m26b_block_norm_dev(None, None, err, 256) == 1 and b"bad arguments" in err.value
+    at = ctypes.addressof(err)
+    assert lib.m26b_linear_dev(None, b"\0" * 256, None, at, 256) == 1 and b"bad handle" in err.value
+    assert lib.m26b_block_norm_dev(None, None, at, 256) == 1 and b"bad arguments" in err.value
     assert lib.m26b_linear_workspace_bytes(None, 5) == 0
     lib.m26b_linear_free(None)
 
