@@ -130,15 +130,15 @@ cudaError_t launch_linear_pair(const m26b_linear* L, const LinearPairMaps& maps,
     return launch_dependent(linear_pair_kernel<PIECES, GATED>, 2 * items < room ? 2 * items : room, kLpThreads, sizeof(LinearPairSmem<PIECES>) + 1024, st,
                             maps, a, m_pairs, items, tile);
 }
-// Whether a request's activations (rows on vector boundaries) are converted inside the product's kernel. Up to 32 tokens (64 that
-// arrive quantised) that hides behind the weights; up to 128 it pays while a CTA has few chunks, since every weight tile repeats
-// it. Measured, inside / staged: 4,096 x 4,096 BF16 32 tokens 8.2 / 9.6 us, 64 10.9 / 8.7, E4M3 64 7.5 / 8.0, 128 11.3 / 10.3;
-// 1,000 x 1,024 (two chunks per CTA) BF16 40 tokens 5.2 / 5.6, 128 8.6 / 8.5, each with one launch less.
+// Whether a request that single CTAs run converts its activations (rows on vector boundaries) inside the product's kernel. Up to 32 tokens
+// (64 that arrive quantised) that hides behind the weights; beyond, it pays while a CTA has few chunks, since every weight tile
+// repeats it. Measured, inside / staged: 4,096 x 4,096 BF16 32 tokens 8.2 / 9.6 us, 64 10.9 / 8.7, E4M3 64 7.5 / 8.0, 128 11.3 /
+// 10.3; 1,000 x 1,024 (two chunks per CTA) BF16 40 tokens 5.2 / 5.6, 128 8.6 / 8.5, each with one launch less.
 bool linear_direct(const m26b_linear* L, bool bf16, uint32_t rows) {
     if (rows <= (bf16 ? 32u : 64u)) return true;
-    if (rows > 128) return false;
-    const uint32_t chunks = L->k_pad / kChunkK, per_cta = chunks >> linear_log_split(L->tiles, uint64_t(L->sms), chunks);
-    return per_cta * rows <= (bf16 ? 256u : 512u);
+    const uint64_t ctas = uint64_t(L->tiles) * ((rows + 127) / 128), sms = uint64_t(L->sms);
+    const uint32_t chunks = L->k_pad / kChunkK, per_cta = chunks >> linear_log_split(ctas, sms, chunks);
+    return ctas <= sms && per_cta * (rows < 128 ? rows : 128) <= (bf16 ? 256u : 512u);
 }
 // Token tile of the CTA-pair kernel for a request, or 0 if single CTAs (which can split K) finish it sooner, by cycles: rounds of
 // items over the GPU x cycles per item. A 128-wide chunk costs a pair 4 x pieces MMAs, each the slower of its math (tile / 2
@@ -187,13 +187,13 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
     const LinearArgs a{L->sf, sf, rows, rows_cap, L->n, L->k_pad / kChunkK, y, y_f32, y_pitch, fault, x, x_scales, x_pitch, L->k};
     TokenMaps mx{};
     cudaError_t e;
-    if (vec && linear_direct(L, bf16, rows)) {
+    const uint32_t pair_tile = linear_pair_tile(L, bf16, rows), tile = pair_tile ? pair_tile : rows <= 64 ? 64u : 128u;
+    if (vec && !pair_tile && linear_direct(L, bf16, rows)) {
         if (rows <= 16) e = launch_linear_tile<16, true>(L, bf16, mx, a, st);
         else if (rows <= 32) e = launch_linear_tile<32, true>(L, bf16, mx, a, st);
         else if (rows <= 64) e = launch_linear_tile<64, true>(L, bf16, mx, a, st);
         else e = launch_linear_tile<128, true>(L, bf16, mx, a, st);
     } else {
-        const uint32_t pair_tile = linear_pair_tile(L, bf16, rows), tile = pair_tile ? pair_tile : rows <= 64 ? 64u : 128u;
         const SplitArgs sp{x, x_scales, x_pitch, rows, L->k, L->k_pad, rows_cap, tile, rows <= 64 ? 1u : 0u, ws, sf};
         // quantised rows on 16-byte boundaries are loaded from where they are
         const bool in_place = !bf16 && xa % 16 == 0 && x_pitch % 16 == 0;

@@ -333,18 +333,18 @@ struct LinearConverter {
     // No more chunks at work than there are stages: a warp that has finished chunk i knows chunks up to i - kStages to be consumed,
     // so with a step of at most kStages the parity it waits for next cannot be that of a stage's use before last.
     static constexpr uint32_t kLanes = kConvWarps / kParts < kStages ? kConvWarps / kParts : kStages;
-    uint32_t row0, first, g, r0, c0, n_chunks;
+    uint32_t row0, first, g, r0, c0, n_chunks, tok0;
     RawX<PIECES> raw[4];
 
-    __device__ __forceinline__ LinearConverter(uint32_t cw, uint32_t lane, uint32_t c_first, uint32_t chunks)
-        : row0(cw % kParts * 8), first(cw / kParts), g(lane & 15u), r0(row0 + (lane >> 4)), c0(c_first), n_chunks(chunks) {}
+    __device__ __forceinline__ LinearConverter(uint32_t cw, uint32_t lane, uint32_t c_first, uint32_t chunks, uint32_t token)
+        : row0(cw % kParts * 8), first(cw / kParts), g(lane & 15u), r0(row0 + (lane >> 4)), c0(c_first), n_chunks(chunks), tok0(token) {}
     __device__ __forceinline__ void request(const LinearArgs& p, uint32_t i) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) raw[v].load(p, r0 + 2 * v, (c0 + i) * kChunkK + g * 8);
+        for (int v = 0; v < 4; ++v) raw[v].load(p, tok0 + r0 + 2 * v, (c0 + i) * kChunkK + g * 8);
     }
     template <class Smem>
     __device__ __forceinline__ void run(const LinearArgs& p, Smem& s, uint32_t lane) {
-        if (row0 >= p.rows || first >= kLanes || first >= n_chunks) return;
+        if (tok0 + row0 >= p.rows || first >= kLanes || first >= n_chunks) return;
         request(p, first);
         for (uint32_t i = first; i < n_chunks; i += kLanes) {
             const uint32_t stage = i % kStages, phase = (i / kStages) & 1u;
@@ -394,7 +394,7 @@ struct LinearConverter {
 // finishing an equal part of the tile's features, so the result does not depend on timing. Token tiles start on multiples of 128
 // (their scale blocks hold 128 tokens): smaller B_ROWS serve requests of at most B_ROWS tokens.
 //
-// DIRECT (up to 128 tokens, rows on 16-byte boundaries): the epilogue warps, idle while the weights stream, turn the activations of
+// DIRECT (few tokens, or few chunks per CTA; rows on 16-byte boundaries): the epilogue warps, idle while the weights stream, turn the activations of
 // each chunk into the pieces in shared memory themselves; no second launch, no workspace. Every weight tile repeats that work, so
 // larger requests stage the pieces once (linear_split_kernel) and fetch them with TMA.
 template <int B_ROWS, int PIECES, bool GATED, bool DIRECT>
@@ -414,7 +414,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     volatile uint32_t* abort_flag = &s.abort_flag;
 
     if (threadIdx.x == 0) {
-        const uint32_t filled = DIRECT ? 1 + (p.rows + 7) / 8 : 1;         // the producer, and the converters that share a chunk
+        const uint32_t filled = DIRECT ? 1 + (n_valid + 7) / 8 : 1;         // the producer, and the converters that share a chunk
         for (int i = 0; i < T::kStages; ++i) { mbar_init(&s.full[i], filled); mbar_init(&s.empty[i], 1); }
         mbar_init(&s.acc_full, 1);
         s.abort_flag = 0;
@@ -513,7 +513,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         tc_fence_after();
         const uint32_t tb = s.tmem_base;
         if constexpr (DIRECT) {
-            LinearConverter<B_ROWS, PIECES> conv(uint32_t(warp - 2), uint32_t(lane), c0, c1 - c0);
+            LinearConverter<B_ROWS, PIECES> conv(uint32_t(warp - 2), uint32_t(lane), c0, c1 - c0, tok0);
             grid_dep_wait();                     // the activations come from the stream's earlier kernels
             conv.run(p, s, uint32_t(lane));
         }

@@ -210,6 +210,25 @@ def test_enough_work_for_cta_pairs(torch, rows, k):
     assert int(run.fault) == 0 and int(gated.fault) == 0
 
 
+@pytest.mark.parametrize("rows", [129, 135, 200, 256, 300, 520, 1000])
+@pytest.mark.parametrize("n,k", [(60, 96), (500, 1024), (130, 2048)])
+def test_several_token_tiles_converted_in_the_kernel(torch, rows, n, k):
+    import mimo26f_afd_b200 as M
+
+    g = gen(torch, rows + n)
+    w, s = make_weights(torch, n, k, g)
+    W = weight_f64(torch, w, s)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(torch.bfloat16)
+    q = torch.randint(0, 127, (rows, k), dtype=torch.uint8, device="cuda", generator=g)
+    xs = torch.randint(110, 130, (rows, k // 32), dtype=torch.uint8, device="cuda", generator=g)
+    run = Runner(torch, M.Linear.new(w, s, n, k), rows)
+    y, bound = product_and_bound(torch, x.double(), W)
+    check(torch, run(x, rows), y, rounded(y, bound, False))
+    y, bound = product_and_bound(torch, e4m3_f64(torch, q, xs), W, quantised=True)
+    check(torch, run(q, rows, x_scales=xs), y, rounded(y, bound, False))
+    assert int(run.fault) == 0
+
+
 def test_cta_pairs_with_many_items_each(torch):
     import mimo26f_afd_b200 as M
 
