@@ -63,10 +63,14 @@ int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool 
 
 uint32_t linear_rows_cap(uint32_t rows) { return ((rows < kLinearPassRows ? rows : kLinearPassRows) + 15) & ~15u; }
 
-// log2 of the CTAs that share a weight tile's K: doubled while the CTAs still fit the SMs at once and each keeps at least two chunks.
-uint32_t linear_log_split(uint64_t ctas, uint64_t room, uint32_t chunks) {
+// log2 of the CTAs that share a weight tile's K (a cluster): doubled while the clusters still run at once and each CTA keeps at least
+// two chunks. A GPC holds whole clusters only: of the 148 SMs, 33 clusters of four run at once and fifteen of eight with one CTA per SM
+// (66 and 32 with two), and what is left would run as a second round (100 tokens, 2,048 x 2,048, sixteen clusters of eight: 15.2 us,
+// of four: 8.3). Powers of two: the divisions that other sizes need cost 0.3 us, more than they gain.
+uint32_t linear_log_split(uint64_t ctas, uint64_t sms, uint32_t per_sm, uint32_t chunks) {
+    const uint64_t slots = sms * per_sm, room[4] = {slots, slots, slots * 892 / 1000, slots * (per_sm == 2 ? 865 : 811) / 1000};
     uint32_t log_split = 0;
-    while (log_split < 3 && (ctas << (log_split + 1)) <= room && chunks >= 4u << log_split) ++log_split;
+    while (log_split < 3 && (ctas << (log_split + 1)) <= room[log_split + 1] && chunks >= 4u << log_split) ++log_split;
     return log_split;
 }
 template <int B_ROWS, int PIECES, bool GATED, bool DIRECT>
@@ -82,7 +86,7 @@ cudaError_t launch_linear(const m26b_linear* L, const TokenMaps& mx, const Linea
         opted.fetch_or(bit, std::memory_order_relaxed);
     }
     const uint32_t feats = GATED ? 64 : kTileM, tiles = (a.n + feats - 1) / feats, tok_tiles = (a.rows + B_ROWS - 1) / B_ROWS;
-    const uint32_t log_split = linear_log_split(uint64_t(tiles) * tok_tiles, uint64_t(L->sms) * T::kCtasPerSm, a.chunks);
+    const uint32_t log_split = linear_log_split(uint64_t(tiles) * tok_tiles, uint64_t(L->sms), T::kCtasPerSm, a.chunks);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(tiles << log_split, tok_tiles); cfg.blockDim = dim3(T::kThreads); cfg.dynamicSmemBytes = size_t(smem); cfg.stream = st;
     cudaLaunchAttribute at[2]{};
@@ -137,7 +141,7 @@ cudaError_t launch_linear_pair(const m26b_linear* L, const LinearPairMaps& maps,
 bool linear_direct(const m26b_linear* L, bool bf16, uint32_t rows) {
     if (rows <= (bf16 ? 32u : 64u)) return true;
     const uint64_t ctas = uint64_t(L->tiles) * ((rows + 127) / 128), sms = uint64_t(L->sms);
-    const uint32_t chunks = L->k_pad / kChunkK, per_cta = chunks >> linear_log_split(ctas, sms, chunks);
+    const uint32_t chunks = L->k_pad / kChunkK, per_cta = chunks >> linear_log_split(ctas, sms, 1, chunks);
     return ctas <= sms && per_cta * (rows < 128 ? rows : 128) <= (bf16 ? 256u : 512u);
 }
 // Token tile of the CTA-pair kernel for a request, or 0 if single CTAs (which can split K) finish it sooner, by cycles: rounds of
@@ -162,7 +166,7 @@ uint32_t linear_pair_tile(const m26b_linear* L, bool bf16, uint32_t rows) {
     for (uint32_t tile = kLpTokens - 16; tile >= 64; tile -= 16)
         if (pair_cost(tile) < cost) { best = tile; cost = pair_cost(tile); }
     const uint64_t single = uint64_t(L->tiles) * ((rows + 127) / 128), sms = uint64_t(L->sms);
-    const uint32_t log_split = linear_log_split(single, sms, uint32_t(chunks));
+    const uint32_t log_split = linear_log_split(single, sms, 1, uint32_t(chunks));
     const uint64_t single_cost = ((single << log_split) + sms - 1) / sms * ((chunks >> log_split) * (bf16 ? 768 : 512) + 4000);
     return pair_cost(best) < single_cost ? best : 0;
 }
