@@ -440,7 +440,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             // the weights depend on no earlier kernel: their first stages are requested before the stream's last one ends
             const uint32_t early = n_chunks < uint32_t(T::kStages) ? n_chunks : uint32_t(T::kStages);
             for (uint32_t i = 0; i < early; ++i) weights(i, i);
-            if constexpr (!DIRECT) grid_dep_wait();
+            grid_dep_wait();
             uint32_t stage = 0, phase = 0;
             for (uint32_t i = 0; i < n_chunks; ++i) {
                 if (i >= early) {
@@ -483,6 +483,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         named_bar_sync(1, 32 + 32 * T::kConvWarps);
         tc_fence_after();
         const uint32_t tb = s.tmem_base;
+        grid_dep_wait();                         // bounded waits start when the stream's earlier kernels have ended, however long they take
         if (elect_one()) {
             const uint32_t idesc0 = idesc_mx(kFmtE2M1, kFmtE4M3, (PIECES - 1) * B_ROWS + n_mma, 0, 0);
             const uint64_t a_desc0 = desc_sw128(smem_u32(s.a[0])), b_desc0 = desc_sw128(smem_u32(s.b[0]));
@@ -512,9 +513,9 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         named_bar_sync(1, 32 + 32 * T::kConvWarps);
         tc_fence_after();
         const uint32_t tb = s.tmem_base;
+        grid_dep_wait();                         // as the MMA warp; and the activations come from the stream's earlier kernels
         if constexpr (DIRECT) {
             LinearConverter<B_ROWS, PIECES> conv(uint32_t(warp - 2), uint32_t(lane), c0, c1 - c0, tok0);
-            grid_dep_wait();                     // the activations come from the stream's earlier kernels
             conv.run(p, s, uint32_t(lane));
         }
         // ------------------------------------------------------------ epilogue, first half: tensor memory -> where it is added
@@ -692,6 +693,7 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issue (first CTA of the pair only)
+        grid_dep_wait();             // bounded waits start when the stream's earlier kernels have ended, however long they take
         if (rank == 0 && elect_one()) {
             uint32_t stage = 0, phase = 0, local = 0, slot = 0;
             bool ok = true;
@@ -732,6 +734,7 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
         // ------------------------------------------------------------ epilogue (both CTAs)
         const uint32_t q = uint32_t(warp) & 3u, col0 = uint32_t(warp - 2) / 4 * 64;      // lane quadrant, first of the warp's 64 tokens
         const uint32_t t_acc = tb + ((q * 32u) << 16) + col0;
+        grid_dep_wait();             // as the MMA warp
         uint32_t local = 0;
         for (uint32_t it = pair_id; it < n_items; it += n_pairs, ++local) {
             const uint32_t m = it % m_pairs, t = it / m_pairs, n_valid = tile_tokens(t), n_mma = (n_valid + 15) & ~15u;

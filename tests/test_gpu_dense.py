@@ -511,6 +511,28 @@ def test_two_streams_with_their_own_workspaces_and_a_replayed_graph(torch):
         assert torch.equal(y, want[i])
 
 
+def test_calls_queued_behind_a_long_kernel(torch):
+    """Everything queued while the stream is busy for longer than the bound of the kernels' own waits."""
+    import mimo26f_afd_b200 as M
+
+    n, k = 4096, 512
+    g = gen(torch, 18)
+    w, s = make_weights(torch, n, k, g)
+    layer = M.Linear.new(w, s, n, k)
+    runs = {rows: (Runner(torch, layer, rows), torch.randn(rows, k, device="cuda", generator=g).to(torch.bfloat16)) for rows in (1, 40, 2000)}
+    want = {rows: r(x, rows).clone() for rows, (r, x) in runs.items()}
+    outs = {rows: torch.zeros(rows, n, device="cuda") for rows in runs}
+    copies = {rows: torch.empty(rows, k, dtype=torch.bfloat16, device="cuda") for rows in runs}
+    torch.cuda.synchronize()
+    torch.cuda._sleep(1_000_000_000)                            # about half a second
+    for rows, (r, x) in runs.items():
+        M.block_norm_dev([x], None, rows, k, h_dtype=0, h_out=copies[rows])      # a copy of x through the norm's kernel
+        r(copies[rows], rows, y=outs[rows])
+    torch.cuda.synchronize()
+    for rows, (r, x) in runs.items():
+        assert int(r.fault) == 0 and torch.equal(copies[rows], x) and torch.equal(outs[rows], want[rows])
+
+
 def test_linear_refusals(torch):
     import mimo26f_afd_b200 as M
 
