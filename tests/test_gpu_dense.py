@@ -620,8 +620,10 @@ def norm_case(torch, rows, width, *, planes=1, y32=False, h32=True, n32=True, w3
     dh = 64 * U * terms
     eps_b = lambda f32: 0.0 if f32 else 2.0**-8  # noqa: E731
     assert bool(((h.double() - want_h).abs() <= dh + eps_b(h32) * (want_h.abs() + dh)).all())
-    r = want_n.abs() / want_h.abs().clamp_min(1e-300)
-    mean_dh = (dh.square().mean(-1, keepdim=True)).sqrt() / (want_h.square().mean(-1, keepdim=True) + 1e-5).sqrt()
+    # n = h w / rms, so an error dh of h is |w| / rms dh of n (also where h itself is zero), beside that of the row's rms
+    rms = (want_h.square().mean(-1, keepdim=True) + 1e-5).sqrt()
+    r = (nw.double().abs() if nw is not None else 1.0) / rms
+    mean_dh = (dh.square().mean(-1, keepdim=True)).sqrt() / rms
     dn = r * dh + (64 * U + mean_dh) * want_n.abs() + 1e-30
     assert bool(((n.double() - want_n).abs() <= dn + eps_b(n32) * (want_n.abs() + dn)).all())
     h.fill_(float("nan"))
