@@ -358,7 +358,7 @@ int m26b_plan_static(const int32_t* ids, const float* weights, uint32_t rows, in
  *   linear_dev: x [rows][k], BF16 or E4M3 with UE8M0 scales per 32 k -> y [rows][n], BF16 (one rounding, nearest even) or
  *              FP32. Only y's n columns of `rows` rows are written. One token to a prefill batch (passes of 8,192; at most
  *              2^31 - 1 rows); 0 rows is no work. BF16 activations are not quantised: a K32 block enters the product as two E4M3
- *              pieces that equal it exactly, save for elements below 2^-14 of the block's largest, which carry an error of
+ *              pieces that equal it exactly, save for elements below 2^-13 of the block's largest, which carry an error of
  *              at most 2^-21 of that largest. Products accumulate in FP32. A row with an infinity, a NaN (or, for E4M3, a NaN
  *              code or scale byte 255) in it is NaN in all its outputs. A row's result does not change with the other rows'
  *              values. Nothing is allocated, nothing is synchronised, and a call can be captured into a graph; the handle
