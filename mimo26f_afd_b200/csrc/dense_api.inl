@@ -148,7 +148,7 @@ bool linear_direct(const m26b_linear* L, bool bf16, uint32_t rows) {
 // items over the GPU x cycles per item. A 128-wide chunk costs a pair 4 x pieces MMAs, each the slower of its math (tile / 2
 // cycles) and of shared memory at 128 B/clk (weight rows 32 cycles, token rows tile / 8, its share of filling the stage); a
 // single CTA of 128 tokens 768 (two pieces) or 512 cycles, shared memory again. The constants are what start, end and
-// hand-over of an item cost. A tile narrower than 256 tokens has to win by a tenth: it is more work in all, and the GPU is at
+// hand-over of an item cost. A tile narrower than the widest has to win by a tenth: it is more work in all, and the GPU is at
 // its power limit. Measured (4,096 x 4,096, pairs / single CTAs): 512 tokens 22.1 / 20.3 us, 768 26.6 / 31.1, E4M3 512 17.9 / 15.0,
 // 1,024 21.5 / 28.9; 1,536 tokens with tiles of 176 / 256: 46.0 / 53.1 us.
 uint32_t linear_pair_tile(const m26b_linear* L, bool bf16, uint32_t rows) {
@@ -161,9 +161,10 @@ uint32_t linear_pair_tile(const m26b_linear* L, bool bf16, uint32_t rows) {
         const uint64_t math = tile / 2, feed = 32 + tile / 8 + (128 + pieces * tile / 2) / (4 * pieces);
         return rounds * (chunks * 4 * pieces * (math > feed ? math : feed) + 2000) + 10000;
     };
-    uint32_t best = kLpTokens;
-    uint64_t cost = pair_cost(kLpTokens) * 9 / 10;
-    for (uint32_t tile = kLpTokens - 16; tile >= 64; tile -= 16)
+    const uint32_t widest = bf16 ? LinearPairTile<2>::kTokens : LinearPairTile<1>::kTokens;
+    uint32_t best = widest;
+    uint64_t cost = pair_cost(widest) * 9 / 10;
+    for (uint32_t tile = widest - 16; tile >= 64; tile -= 16)
         if (pair_cost(tile) < cost) { best = tile; cost = pair_cost(tile); }
     const uint64_t single = uint64_t(L->tiles) * ((rows + 127) / 128), sms = uint64_t(L->sms);
     const uint32_t log_split = linear_log_split(single, sms, 1, uint32_t(chunks));

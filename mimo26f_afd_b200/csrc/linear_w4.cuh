@@ -577,16 +577,25 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 }
 
 // ---- the product on CTA pairs (prefill) -----------------------------------------------------------------------------
-// cta_group::2: two CTAs of a cluster run one MMA of M = 256 (128 weight rows each) x N = `tile` tokens (at most 256), half of the token
-// rows in each CTA's shared memory. What bounds a block-scaled MMA at prefill is shared memory, which feeds the operands (128 B/clk) and
-// takes the loads: per 128-wide chunk and CTA this shape reads PIECES x 32 KB and fills 16 + PIECES x 16 KB in PIECES x 512 cycles of
-// math, 112 B/clk with two pieces; 128 tokens wide it would be 144, a single CTA of 128 x 128 tokens 192. The pieces
-// accumulate one after the other into the same 256 columns, which leaves the other half of tensor memory to the scales.
+// cta_group::2: two CTAs of a cluster run one MMA of M = 256 (128 weight rows each) x N = `tile` tokens (at most 256 with one piece, 224
+// with two), half of the token rows in each CTA's shared memory. What bounds a block-scaled MMA at prefill is shared memory, which feeds the
+// operands (128 B/clk) and takes the loads: per 128-wide chunk and CTA, 224 tokens of two pieces read 60 KB and fill 44 KB in 896 cycles
+// of math, 119 B/clk; 128 tokens wide it would be 144, a single CTA of 128 x 128 tokens 192.
+// Each piece has accumulator columns of its own, added once in the epilogue. The tensor core truncates its running sum to FP32 after every
+// MMA. The leading pieces' products lie on a coarse grid, so that little falls off; with the second pieces' sixteen times finer
+// products in the same column every step loses a part of a unit in the last place, towards zero (2,048 tokens, 4,096 x 4,096, FP32
+// out: off by 8.8e-7 of the result with shared columns). Two sets of 224 columns leave 64 to the scales.
 // The accumulators are pulled into registers (64 per thread) and handed back before the epilogue's math, so that the next
 // item's MMAs run meanwhile. Barriers as in gemm_mx_pair.cuh: loads of both CTAs report to the first CTA's `full`.
-constexpr uint32_t kLpTokens = 256;                        // widest token tile
+constexpr uint32_t kLpMaxTokens = 256;
 constexpr int kLpEpiWarps = 16, kLpThreads = 64 + 32 * kLpEpiWarps;
-constexpr uint32_t kLpSfSlots = 8, kLpSfStride = 32;       // scale slots above the accumulators: 4 columns of weights, 8 per piece of tokens
+constexpr uint32_t kLpSfStride = 32;                       // a scale slot: 4 columns of weights, 8 per piece of tokens
+template <int PIECES>
+struct LinearPairTile {
+    static constexpr uint32_t kTokens = PIECES == 2 ? 224 : kLpMaxTokens;       // widest token tile; a piece's accumulator columns
+    static constexpr uint32_t kSf = PIECES * kTokens, kSfSlots = (kTmemCols - kSf) / kLpSfStride;    // scale slots above the accumulators
+    static_assert(kSfSlots >= 2 && 4 + 8 * PIECES <= kLpSfStride, "consecutive chunks use different slots");
+};
 
 struct LinearPairMaps {
     CUtensorMap w;          // weight rows, box 128
@@ -597,8 +606,9 @@ struct LinearPairMaps {
 template <int PIECES>
 struct LinearPairSmem {
     static constexpr int kStages = PIECES == 2 ? 4 : 6;
+    static constexpr uint32_t kPieceBytes = LinearPairTile<PIECES>::kTokens / 2 * 128;
     alignas(1024) uint8_t a[kStages][kTileM * 128];
-    alignas(1024) uint8_t b[kStages][PIECES * (kLpTokens / 2) * 128];
+    alignas(1024) uint8_t b[kStages][PIECES * kPieceBytes];
     alignas(128) uint8_t sfa[kStages][kScaleBlockBytes];
     alignas(128) uint8_t sfb[kStages][2 * PIECES * kScaleBlockBytes];       // [128-token run of the tile][piece]
     uint64_t full[kStages], empty[kStages], acc_full, acc_empty;
@@ -611,6 +621,7 @@ template <int PIECES, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
 linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs p, const uint32_t m_pairs, const uint32_t n_items, const uint32_t tile_n) {
     using Smem = LinearPairSmem<PIECES>;
+    using T = LinearPairTile<PIECES>;
     constexpr uint32_t kStages = Smem::kStages;
     extern __shared__ uint8_t smem_raw[];
     Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -673,7 +684,7 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
                         for (uint32_t b = 0; b < 5; ++b) {
                             const uint32_t box = 128u >> b;
                             if (half - r >= box) {
-                                tma_load_2d_pair(s.b[stage] + (piece * (kLpTokens / 2) + r) * 128, &maps.tok[b], int(c * kChunkK),
+                                tma_load_2d_pair(s.b[stage] + piece * Smem::kPieceBytes + r * 128, &maps.tok[b], int(c * kChunkK),
                                                  int(piece * p.rows_cap + t * tile_n + rank * half + r), bar);
                                 r += box;
                             }
@@ -707,8 +718,8 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
                 for (uint32_t c = 0; c < p.chunks; ++c) {
                     if (!mbar_wait(&s.full[stage], phase, abort_flag)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t t_sf = tb + kLpTokens + slot * kLpSfStride;
-                    slot = (slot + 1) % kLpSfSlots;
+                    const uint32_t t_sf = tb + T::kSf + slot * kLpSfStride;
+                    slot = (slot + 1) % T::kSfSlots;
                     tc_cp_scales_pair(t_sf, sfa_desc0 + stage * (sizeof(s.sfa[0]) >> 4));
                     const uint64_t sfb_d = sfb_desc0 + stage * (sizeof(s.sfb[0]) >> 4);
 #pragma unroll
@@ -721,8 +732,8 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
                     for (uint32_t piece = 0; piece < PIECES; ++piece)
 #pragma unroll
                         for (uint32_t kb = 0; kb < 4; ++kb)
-                            tc_mma_mx_pair(tb, ad + 2 * kb, bd + piece * (((kLpTokens / 2) * 128) >> 4) + 2 * kb, idesc0 | (kb << 4) | (kb << 29), t_sf,
-                                           t_sf + 4 + 8 * piece, (c | piece | kb) ? 1u : 0u);
+                            tc_mma_mx_pair(tb + piece * T::kTokens, ad + 2 * kb, bd + piece * (Smem::kPieceBytes >> 4) + 2 * kb, idesc0 | (kb << 4) | (kb << 29),
+                                           t_sf, t_sf + 4 + 8 * piece, (c | kb) ? 1u : 0u);
                     tc_commit_pair(&s.empty[stage]);
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
@@ -748,6 +759,17 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
 #pragma unroll
             for (uint32_t g = 0; g < 4; ++g)
                 if (col0 + 16 * g < n_mma) tmem_ld16(t_acc + 16 * g, r[g]);
+            if constexpr (PIECES == 2) {
+#pragma unroll
+                for (uint32_t g = 0; g < 4; ++g) {
+                    if (col0 + 16 * g >= n_mma) continue;
+                    uint32_t l[16];
+                    tmem_ld16(t_acc + T::kTokens + 16 * g, l);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) r[g][j] = __float_as_uint(__uint_as_float(r[g][j]) + __uint_as_float(l[j]));
+                }
+            }
             tmem_wait_ld();
             tc_fence_before();
             __syncwarp();

@@ -1,0 +1,54 @@
+"""The dense operators where FP32 itself decides: sums that are exact by construction, the activation over the whole range of its
+argument, norm factors near the ends of the range. Formulas in 64 bits; helpers and the derivation of the common bounds are
+test_gpu_dense's."""
+import pytest
+import test_gpu_dense as D
+
+pytestmark = pytest.mark.gpu
+
+U = D.U
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+
+    assert torch.cuda.is_available(), "these tests need the GPU box"
+    return torch
+
+
+@pytest.mark.parametrize("rows,n,k,fine,split", [(20, 200, 512, 7, 8), (300, 1000, 1024, 6, 8), (2048, 4096, 4096, 4, 1), (300, 4096, 16384, 2, 1), (273, 11344, 2048, 5, 1)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_sums_that_fit_fp32_are_exact(torch, rows, n, k, fine, split, gated):
+    """Activations 128..255 (eight significant bits), weights 0.5 and mostly 6, every other K32 block scaled by 2^-fine. The leading pieces'
+    products are multiples of 8 * 2^-fine and their sums fit 24 bits, the second pieces' are multiples of 2^-fine / 2 and theirs fit too: both
+    are exact in FP32, so what comes out is the true sum, rounded once. As one running sum they would need 26 bits and lose some
+    in every step. Gated: a gate of 256 makes the activation the identity (e^-256 is nothing beside 1)."""
+    import mimo26f_afd_b200 as M
+
+    step = 2.0**-fine
+    assert k / 2 * 6 * 256 * (1 + step) < 2**24 * 8 * step and k * 6 * 8 < 2**24 * step / 2     # 256: a leading piece rounds up to it
+    g = D.gen(torch, rows + k)
+    x = torch.randint(128, 256, (rows, k), device="cuda", generator=g)
+    x[:, ::32] = 255
+    x = x.to(torch.bfloat16)
+    w = torch.where(torch.rand(n, k, device="cuda", generator=g) < 0.1, 1, 7).to(torch.uint8)            # E2M1 codes of 0.5 and 6
+    w = w[:, 0::2] | w[:, 1::2] << 4
+    s = torch.full((n, k // 32), 127, dtype=torch.uint8, device="cuda")
+    s[:, 1::2] -= fine
+    want = x.double() @ D.weight_f64(torch, w, s).T                        # exact in 64 bits
+    layer = M.Linear.new(w, s, n, k)
+    if gated:
+        gw = torch.zeros_like(w)                                           # one weight of 1 on the block's first activation: 255
+        gw[:, 0] = 2
+        layer = M.Linear.gated(gw, torch.full_like(s, 127), w, s, n, k)
+        want = want * 255
+    run = D.Runner(torch, layer, rows)
+    y = run(x, rows)
+    torch.cuda.synchronize()
+    ulp = torch.exp2(torch.floor(torch.log2(want)) - 23)
+    # half a unit; where K is split (at most eight ways), one for each partial result and one for each sum of two; the activation 4 units
+    allowed = (2 * split - 1) / 2 + (4 if gated else 0)
+    off = (y.double() - want).abs() / ulp
+    assert float(off.max()) <= allowed, f"{float(off.max()):.3g} units in the last place"
+    assert int(run.fault) == 0
