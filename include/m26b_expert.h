@@ -369,6 +369,9 @@ int m26b_linear_new(const uint8_t* w, const uint8_t* s, uint32_t n, uint32_t k, 
 int m26b_linear_new_gated(const uint8_t* gate_w, const uint8_t* gate_s, const uint8_t* up_w, const uint8_t* up_s, uint32_t n, uint32_t k,
                           m26b_linear** out, char* err, size_t errlen);
 void m26b_linear_free(m26b_linear* l);
+/* Bound of a call's wait for its own tensor-core work, in microseconds of the nominal clock (default about 200,000; at least 1; return 1
+ * for 0 or a NULL handle). Later calls on the handle that exceed it finish with code 3 in their fault word. */
+int m26b_linear_set_wait_us(m26b_linear* l, uint32_t us);
 uint64_t m26b_linear_workspace_bytes(const m26b_linear* l, uint32_t rows);
 typedef struct m26b_linear_args {
     const void* x;              /* device [rows][k], rows x_pitch elements apart (0: dense) */

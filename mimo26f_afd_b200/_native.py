@@ -23,7 +23,7 @@ SYMBOLS = (
     "m26b_ffn_tp", "m26b_ffn_tp_dev", "m26b_ep_ffn", "m26b_layer_image", "m26b_layer_new_from_checkpoint_ep_replicated",
     "m26b_frame_request_bytes", "m26b_frame_return_bytes", "m26b_frame_crc32c", "m26b_frame_crc32c_table", "m26b_frame_encode_request",
     "m26b_serve_frame", "m26b_frame_parse_return", "m26b_frame_check_request",
-    "m26b_linear_new", "m26b_linear_new_gated", "m26b_linear_free", "m26b_linear_workspace_bytes", "m26b_linear_dev",
+    "m26b_linear_new", "m26b_linear_new_gated", "m26b_linear_free", "m26b_linear_set_wait_us", "m26b_linear_workspace_bytes", "m26b_linear_dev",
     "m26b_block_norm_dev",
 )
 
@@ -70,6 +70,7 @@ def lib() -> C.CDLL:
     L.m26b_linear_new_gated.argtypes = [u8p, u8p, u8p, u8p, C.c_uint32, C.c_uint32, C.POINTER(vp), *err]
     L.m26b_linear_free.argtypes = [vp]
     L.m26b_linear_free.restype = None
+    L.m26b_linear_set_wait_us.argtypes = [vp, C.c_uint32]
     L.m26b_linear_workspace_bytes.argtypes = [vp, C.c_uint32]
     L.m26b_linear_workspace_bytes.restype = C.c_uint64
     # the argument records as packed bytes and the error buffer as an address (dense.py): calls of a decode step, several per layer

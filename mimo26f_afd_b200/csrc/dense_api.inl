@@ -9,6 +9,8 @@ struct m26b_linear {
     bool gated = false;
     int device = 0, sms = 0;
     uint32_t tiles = 0;                         // 128-row tiles of the image (even)
+    int khz = 0;                                // nominal SM clock
+    long long wait_cycles = kWaitCycles;        // bound of the epilogues' wait for their accumulators
     CUtensorMap map_w, map_sf;
 };
 
@@ -40,7 +42,9 @@ int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool 
     };
     cudaError_t e = cudaGetDevice(&L->device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&L->sms, cudaDevAttrMultiProcessorCount, L->device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&L->khz, cudaDevAttrClockRate, L->device);
     if (e != cudaSuccess) return fail("m26b linear device", e);
+    if (L->khz <= 0) L->khz = 1965000;
     if ((e = cudaDeviceSynchronize()) != cudaSuccess) return fail("m26b linear sync", e);      // the source may come from any stream
     void* mem = nullptr;
     if ((e = cudaMalloc(&mem, w_bytes)) != cudaSuccess) return fail("m26b linear weights alloc", e);
@@ -189,7 +193,8 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
     const uintptr_t xa = reinterpret_cast<uintptr_t>(x);
     const int vec = bf16 ? (xa % 16 == 0 && x_pitch % 8 == 0) : (xa % 8 == 0 && x_pitch % 8 == 0);
     uint8_t* sf = ws + uint64_t(pieces) * rows_cap * L->k_pad;
-    const LinearArgs a{L->sf, sf, rows, rows_cap, L->n, L->k_pad / kChunkK, y, y_f32, y_pitch, fault, x, x_scales, x_pitch, L->k};
+    const LinearArgs a{L->sf, sf, rows, rows_cap, L->n, L->k_pad / kChunkK, y, y_f32, y_pitch, fault, x, x_scales, x_pitch, L->k,
+                       L->wait_cycles};
     TokenMaps mx{};
     cudaError_t e;
     const uint32_t pair_tile = linear_pair_tile(L, bf16, rows), tile = pair_tile ? pair_tile : rows <= 64 ? 64u : 128u;
@@ -324,6 +329,11 @@ void m26b_linear_free(m26b_linear* l) {
     if (l->w) cudaFree(l->w);
     if (l->sf) cudaFree(l->sf);
     delete l;
+}
+int m26b_linear_set_wait_us(m26b_linear* l, uint32_t us) {
+    if (!l || !us) return 1;
+    l->wait_cycles = (long long)us * l->khz / 1000;
+    return 0;
 }
 uint64_t m26b_linear_workspace_bytes(const m26b_linear* l, uint32_t rows) {
     if (!l || !rows) return 0;

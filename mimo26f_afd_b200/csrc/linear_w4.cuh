@@ -235,7 +235,24 @@ struct LinearArgs {
     const uint8_t* x_scales;
     uint64_t x_pitch;
     uint32_t k;
+    long long wait_cycles;       // bound of the epilogue's wait for its accumulators
 };
+
+// An epilogue warp's wait for finished accumulators. If it takes longer than p.wait_cycles, or another role has given up, that is
+// reported and the answer is false; what is under way is waited for all the same (with the common bound), so that nothing
+// of the tensor core or the copies is in flight when the kernel ends.
+__device__ __forceinline__ bool acc_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, const LinearArgs& p) {
+    const long long t0 = clock64();
+    bool done, in_time;
+    do {
+        done = mbar_try_wait(bar, parity);
+        in_time = clock64() - t0 <= p.wait_cycles;
+    } while (!done && in_time && !*abort_flag);
+    if (done && in_time) return true;
+    atomicOr(p.fault, uint32_t(kFaultPipeline));
+    if (!done) mbar_wait(bar, parity, abort_flag);
+    return false;
+}
 
 __device__ __forceinline__ float silu_gate(float g, float u) {
     // g / (1 + e^-g) * u without a positive exponential; infinities of g give +inf * u and -0 * u
@@ -521,7 +538,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         // ------------------------------------------------------------ epilogue, first half: tensor memory -> where it is added
         const uint32_t q = uint32_t(warp) & 3u;            // lane quadrant; the quadrant's warps take sixteen tokens in turn
         const uint32_t row = q * 32u + lane;               // weight row of the tile
-        const bool ok = mbar_wait(&s.acc_full, 0, abort_flag);
+        const bool ok = acc_wait(&s.acc_full, 0, abort_flag, p);
         __syncwarp();
         if (split > 1) cluster_wait();
         if (__all_sync(0xffffffffu, ok)) {
@@ -749,11 +766,8 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
         uint32_t local = 0;
         for (uint32_t it = pair_id; it < n_items; it += n_pairs, ++local) {
             const uint32_t m = it % m_pairs, t = it / m_pairs, n_valid = tile_tokens(t), n_mma = (n_valid + 15) & ~15u;
-            const bool got = mbar_wait(&s.acc_full, local & 1u, abort_flag);
-            if (!__all_sync(0xffffffffu, got)) {
-                if (lane == 0) atomicOr(p.fault, uint32_t(kFaultPipeline));
-                break;
-            }
+            const bool got = __all_sync(0xffffffffu, acc_wait(&s.acc_full, local & 1u, abort_flag, p));
+            if (!got && __any_sync(0xffffffffu, *abort_flag != 0)) break;        // the pipeline stands still
             tc_fence_after();
             uint32_t r[4][16];
 #pragma unroll
@@ -774,6 +788,7 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(cluster_map(smem_u32(&s.acc_empty), 0));
+            if (!got) continue;
             const uint32_t tile = 2 * m + rank, feat = GATED ? tile * 64 + q * 16 + (lane & 15) : tile * kTileM + q * 32 + lane;
 #pragma unroll
             for (uint32_t g = 0; g < 4; ++g)

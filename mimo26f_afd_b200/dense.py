@@ -70,6 +70,12 @@ class Linear:
         """Device bytes ``linear_dev`` needs for ``rows`` tokens."""
         return int(_native.lib().m26b_linear_workspace_bytes(self._h, rows))
 
+    def set_wait_us(self, us: int) -> None:
+        """Bound of a call's wait for its own tensor-core work (default about 200,000 us); later calls that exceed it put code 3
+        into their fault word."""
+        if not 0 < us < 1 << 32 or _native.lib().m26b_linear_set_wait_us(self._h, us):
+            raise ExpertError(1, "m26b linear: bad wait bound or handle")
+
     def close(self) -> None:
         if self._h:
             _native.lib().m26b_linear_free(self._h)

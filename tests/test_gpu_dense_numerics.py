@@ -52,3 +52,29 @@ def test_sums_that_fit_fp32_are_exact(torch, rows, n, k, fine, split, gated):
     off = (y.double() - want).abs() / ulp
     assert float(off.max()) <= allowed, f"{float(off.max()):.3g} units in the last place"
     assert int(run.fault) == 0
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,n,k", [(100, 4096, 16384), (100, 20000, 4096), (2048, 4096, 4096), (700, 9600, 4096)])
+def test_a_wait_that_runs_out_is_reported(torch, rows, n, k, gated):
+    """A bound of a microsecond on accumulators that take ten and more: K split over a cluster, single CTAs, CTA pairs with one and with several
+    items each. The kernel ends, the fault word says so, and the handle works on."""
+    import mimo26f_afd_b200 as M
+
+    g = D.gen(torch, rows)
+    w, s = D.make_weights(torch, n, k, g)
+    layer = M.Linear.gated(w, s, w, s, n, k) if gated else M.Linear.new(w, s, n, k)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(torch.bfloat16)
+    run = D.Runner(torch, layer, rows)
+    want = run(x, rows).clone()
+    torch.cuda.synchronize()
+    assert int(run.fault) == 0
+    layer.set_wait_us(1)
+    run(x, rows)
+    torch.cuda.synchronize()
+    assert int(run.fault) == 3
+    layer.set_wait_us(200_000)
+    run.fault.zero_()
+    got = run(x, rows)
+    torch.cuda.synchronize()
+    assert int(run.fault) == 0 and torch.equal(got, want)
