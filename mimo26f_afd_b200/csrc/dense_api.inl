@@ -3,6 +3,8 @@
 #pragma once
 #include <new>
 
+#include "linear_rules.h"
+
 struct m26b_linear {
     uint8_t *w = nullptr, *sf = nullptr;        // weight image (linear_w4.cuh)
     uint32_t n = 0, k = 0, k_pad = 0;
@@ -16,9 +18,10 @@ struct m26b_linear {
 
 namespace {
 
+static_assert(linear_widest_pair_tile(true) == LinearPairTile<2>::kTokens && linear_widest_pair_tile(false) == LinearPairTile<1>::kTokens &&
+              kChunkK == 128 && kScaleBlockBytes == 512, "linear_rules.h knows the kernels' widest tiles, a chunk and a scale block");
 constexpr uint32_t kLinearMaxDim = 1u << 20;
 constexpr uint32_t kDenseMaxRows = 0x7fffffffu;
-constexpr uint32_t kLinearPassRows = 8192;      // tokens per pass: bounds the workspace at 2 x 8192 x k bytes
 
 int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool gated, uint32_t n, uint32_t k, m26b_linear** out, char* err,
                size_t errlen) {
@@ -65,18 +68,6 @@ int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool 
     return 0;
 }
 
-uint32_t linear_rows_cap(uint32_t rows) { return ((rows < kLinearPassRows ? rows : kLinearPassRows) + 15) & ~15u; }
-
-// log2 of the CTAs that share a weight tile's K (a cluster): doubled while the clusters still run at once and each CTA keeps at least
-// two chunks. A GPC holds whole clusters only: of the 148 SMs, 33 clusters of four run at once and fifteen of eight with one CTA per SM
-// (66 and 32 with two), and what is left would run as a second round (100 tokens, 2,048 x 2,048, sixteen clusters of eight: 15.2 us,
-// of four: 8.3). Powers of two: the divisions that other sizes need cost 0.3 us, more than they gain.
-uint32_t linear_log_split(uint64_t ctas, uint64_t sms, uint32_t per_sm, uint32_t chunks) {
-    const uint64_t slots = sms * per_sm, room[4] = {slots, slots, slots * 892 / 1000, slots * (per_sm == 2 ? 865 : 811) / 1000};
-    uint32_t log_split = 0;
-    while (log_split < 3 && (ctas << (log_split + 1)) <= room[log_split + 1] && chunks >= 4u << log_split) ++log_split;
-    return log_split;
-}
 template <int B_ROWS, int PIECES, bool GATED, bool DIRECT>
 cudaError_t launch_linear(const m26b_linear* L, const TokenMaps& mx, const LinearArgs& a, cudaStream_t st) {
     using T = LinearTile<B_ROWS, PIECES>;
@@ -131,6 +122,10 @@ int linear_pair_ctas(const m26b_linear* L) {
     mine.store(ctas + 1, std::memory_order_relaxed);
     return ctas;
 }
+uint32_t linear_pair_ctas(const m26b_linear* L, bool bf16) {
+    if (L->gated) return uint32_t(bf16 ? linear_pair_ctas<2, true>(L) : linear_pair_ctas<1, true>(L));
+    return uint32_t(bf16 ? linear_pair_ctas<2, false>(L) : linear_pair_ctas<1, false>(L));
+}
 template <int PIECES, bool GATED>
 cudaError_t launch_linear_pair(const m26b_linear* L, const LinearPairMaps& maps, const LinearArgs& a, uint32_t tile, cudaStream_t st) {
     const uint32_t m_pairs = L->tiles / 2, items = m_pairs * ((a.rows + tile - 1) / tile);
@@ -138,44 +133,6 @@ cudaError_t launch_linear_pair(const m26b_linear* L, const LinearPairMaps& maps,
     return launch_dependent(linear_pair_kernel<PIECES, GATED>, 2 * items < room ? 2 * items : room, kLpThreads, sizeof(LinearPairSmem<PIECES>) + 1024, st,
                             maps, a, m_pairs, items, tile);
 }
-// Whether a request that single CTAs run converts its activations (rows on vector boundaries) inside the product's kernel. Up to 32 tokens
-// (64 that arrive quantised) that hides behind the weights; beyond, it pays while a CTA has few chunks, since every weight tile
-// repeats it. Measured, inside / staged: 4,096 x 4,096 BF16 32 tokens 8.2 / 9.6 us, 64 10.9 / 8.7, E4M3 64 7.5 / 8.0, 128 11.3 /
-// 10.3; 1,000 x 1,024 (two chunks per CTA) BF16 40 tokens 5.2 / 5.6, 128 8.6 / 8.5, each with one launch less.
-bool linear_direct(const m26b_linear* L, bool bf16, uint32_t rows) {
-    if (rows <= (bf16 ? 32u : 64u)) return true;
-    const uint64_t ctas = uint64_t(L->tiles) * ((rows + 127) / 128), sms = uint64_t(L->sms);
-    const uint32_t chunks = L->k_pad / kChunkK, per_cta = chunks >> linear_log_split(ctas, sms, 1, chunks);
-    return ctas <= sms && per_cta * (rows < 128 ? rows : 128) <= (bf16 ? 256u : 512u);
-}
-// Token tile of the CTA-pair kernel for a request, or 0 if single CTAs (which can split K) finish it sooner, by cycles: rounds of
-// items over the GPU x cycles per item. A 128-wide chunk costs a pair 4 x pieces MMAs, each the slower of its math (tile / 2
-// cycles) and of shared memory at 128 B/clk (weight rows 32 cycles, token rows tile / 8, its share of filling the stage); a
-// single CTA of 128 tokens 768 (two pieces) or 512 cycles, shared memory again. The constants are what start, end and
-// hand-over of an item cost. A tile narrower than the widest has to win by a tenth: it is more work in all, and the GPU is at
-// its power limit. Measured (4,096 x 4,096, pairs / single CTAs): 512 tokens 22.1 / 20.3 us, 768 26.6 / 31.1, E4M3 512 17.9 / 15.0,
-// 1,024 21.5 / 28.9; 1,536 tokens with tiles of 176 / 256: 46.0 / 53.1 us.
-uint32_t linear_pair_tile(const m26b_linear* L, bool bf16, uint32_t rows) {
-    if (rows <= 128) return 0;
-    const int ctas = L->gated ? (bf16 ? linear_pair_ctas<2, true>(L) : linear_pair_ctas<1, true>(L)) : (bf16 ? linear_pair_ctas<2, false>(L) : linear_pair_ctas<1, false>(L));
-    if (ctas < 2) return 0;
-    const uint64_t pairs = uint64_t(ctas) / 2, m_pairs = L->tiles / 2, chunks = L->k_pad / kChunkK, pieces = bf16 ? 2 : 1;
-    const auto pair_cost = [&](uint32_t tile) {
-        const uint64_t rounds = (m_pairs * ((rows + tile - 1) / tile) + pairs - 1) / pairs;
-        const uint64_t math = tile / 2, feed = 32 + tile / 8 + (128 + pieces * tile / 2) / (4 * pieces);
-        return rounds * (chunks * 4 * pieces * (math > feed ? math : feed) + 2000) + 10000;
-    };
-    const uint32_t widest = bf16 ? LinearPairTile<2>::kTokens : LinearPairTile<1>::kTokens;
-    uint32_t best = widest;
-    uint64_t cost = pair_cost(widest) * 9 / 10;
-    for (uint32_t tile = widest - 16; tile >= 64; tile -= 16)
-        if (pair_cost(tile) < cost) { best = tile; cost = pair_cost(tile); }
-    const uint64_t single = uint64_t(L->tiles) * ((rows + 127) / 128), sms = uint64_t(L->sms);
-    const uint32_t log_split = linear_log_split(single, sms, 1, uint32_t(chunks));
-    const uint64_t single_cost = ((single << log_split) + sms - 1) / sms * ((chunks >> log_split) * (bf16 ? 768 : 512) + 4000);
-    return pair_cost(best) < single_cost ? best : 0;
-}
-
 cudaError_t launch_stage(void (*kernel)(SplitArgs), dim3 grid, const SplitArgs& a, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid; cfg.blockDim = dim3(256); cfg.stream = st;
@@ -197,8 +154,9 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
                        L->wait_cycles};
     TokenMaps mx{};
     cudaError_t e;
-    const uint32_t pair_tile = linear_pair_tile(L, bf16, rows), tile = pair_tile ? pair_tile : rows <= 64 ? 64u : 128u;
-    if (vec && !pair_tile && linear_direct(L, bf16, rows)) {
+    const LinearShape shape{L->tiles, L->k_pad / kChunkK, uint32_t(L->sms)};
+    const uint32_t pair_tile = rows <= 128 ? 0 : linear_pair_tile(shape, linear_pair_ctas(L, bf16), bf16, rows), tile = pair_tile ? pair_tile : rows <= 64 ? 64u : 128u;
+    if (vec && !pair_tile && linear_direct(shape, bf16, rows)) {
         if (rows <= 16) e = launch_linear_tile<16, true>(L, bf16, mx, a, st);
         else if (rows <= 32) e = launch_linear_tile<32, true>(L, bf16, mx, a, st);
         else if (rows <= 64) e = launch_linear_tile<64, true>(L, bf16, mx, a, st);
@@ -226,7 +184,7 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
             LinearPairMaps pm{};
             pm.w = L->map_w; pm.sfa = L->map_sf;
             const uint32_t blocks = (tile > 128 ? 2 : 1) * pieces;
-            maps_ok = boxes(pm.tok, 5) && make_sf_map(&pm.sfb, sf, uint64_t((rows + tile - 1) / tile) * a.chunks * blocks, blocks);
+            maps_ok = boxes(pm.tok, 5) && make_sf_map(&pm.sfb, sf, linear_scale_blocks(rows, tile, pieces) * a.chunks, blocks);
             if (maps_ok) {
                 if (L->gated) e = bf16 ? launch_linear_pair<2, true>(L, pm, a, tile, st) : launch_linear_pair<1, true>(L, pm, a, tile, st);
                 else e = bf16 ? launch_linear_pair<2, false>(L, pm, a, tile, st) : launch_linear_pair<1, false>(L, pm, a, tile, st);
@@ -336,10 +294,7 @@ int m26b_linear_set_wait_us(m26b_linear* l, uint32_t us) {
     return 0;
 }
 uint64_t m26b_linear_workspace_bytes(const m26b_linear* l, uint32_t rows) {
-    if (!l || !rows) return 0;
-    const uint64_t cap = linear_rows_cap(rows);
-    // two pieces of codes, and scale blocks: two per 128-token run, of which a tile of 64..256 tokens has at most (rows / 64 + 1)
-    return 2 * (cap * l->k_pad + (cap / 64 + 1) * (l->k_pad / kChunkK) * kScaleBlockBytes);
+    return l ? linear_workspace(l->k_pad, rows) : 0;
 }
 int m26b_linear_dev(const m26b_linear* l, const m26b_linear_args* args, void* stream, char* err, size_t errlen) {
     if (!l || !args || !(args->x_dtype == 0 || args->x_dtype == 2) || args->y_dtype < 0 || args->y_dtype > 1 || args->reserved) {

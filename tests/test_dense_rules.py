@@ -16,3 +16,69 @@ def test_the_wait_bound_is_checked():
         with pytest.raises(M.ExpertError) as e:
             Handle().set_wait_us(us)
         assert e.value.code == 1
+
+
+@pytest.fixture(scope="module")
+def rules(tmp_path_factory):
+    """linear_rules.h, compiled for the host."""
+    import ctypes as C
+    import subprocess
+
+    from conftest import ROOT
+
+    d = tmp_path_factory.mktemp("rules")
+    (d / "rules.cpp").write_text('''#include "linear_rules.h"
+using namespace m26b;
+extern "C" {
+uint64_t workspace(uint32_t k_pad, uint32_t rows) { return linear_workspace(k_pad, rows); }
+uint64_t blocks(uint32_t rows, uint32_t tile, uint32_t pieces) { return linear_scale_blocks(rows, tile, pieces); }
+uint32_t pair_tile(uint32_t tiles, uint32_t chunks, uint32_t sms, uint32_t ctas, int bf16, uint32_t rows) { return linear_pair_tile({tiles, chunks, sms}, ctas, bf16, rows); }
+uint32_t widest(int bf16) { return linear_widest_pair_tile(bf16); }
+}
+''')
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", f"{ROOT}/mimo26f_afd_b200/csrc", "-o", str(d / "rules.so"), str(d / "rules.cpp")], check=True)
+    lib = C.CDLL(str(d / "rules.so"))
+    lib.workspace.restype = lib.blocks.restype = C.c_uint64
+    lib.pair_tile.restype = lib.widest.restype = C.c_uint32
+    return lib
+
+
+def test_every_token_tile_fits_the_workspace(rules):
+    """Not only the tiles that the costs choose: the codes of both pieces and, behind them, the last scale block that the staging kernel writes and
+    the last that a tensor map covers, for every number of tokens and every tile a kernel can run."""
+    import numpy as np
+
+    chunks = 3
+    k_pad = 128 * chunks
+    last = 0
+    sizes = []
+    for rows in range(1, 8193):
+        size = rules.workspace(k_pad, rows)
+        assert size >= last
+        last = size
+        sizes.append(size)
+    assert rules.workspace(k_pad, 0) == 0 and rules.workspace(k_pad, 1 << 20) == last
+    sizes = np.array(sizes)
+    rows = np.arange(1, 8193)
+    for pieces in (1, 2):
+        codes = pieces * ((rows + 15) // 16 * 16) * k_pad
+        for tile in range(64, rules.widest(pieces == 2) + 1, 16):
+            runs = 2 if tile > 128 else 1
+            used = rows > 64 if tile != 64 else rows > 0          # up to 64 tokens always take tiles of 64
+            covered = np.array([rules.blocks(int(r), tile, pieces) for r in rows]) * chunks
+            t, r = (rows - 1) // tile, (rows - 1) % tile          # place of the last token's scales, as linear_split_kernel computes it
+            joint = rows <= 64
+            written = np.where(joint, chunks, (t * chunks + chunks - 1) * runs * pieces + (r >> 7) * pieces + pieces)
+            assert (written <= covered)[used].all()
+            assert (codes + covered * 512 <= sizes)[used].all(), (pieces, tile)
+
+
+def test_the_chosen_tiles_are_tiles_of_the_kernel(rules):
+    import random
+
+    rng = random.Random(7)
+    for _ in range(20000):
+        bf16, rows = rng.random() < 0.5, int(2 ** rng.uniform(0, 13))
+        tile = rules.pair_tile(2 * int(2 ** rng.uniform(0, 9)), int(2 ** rng.uniform(0, 8)), 148, 148, bf16, rows)
+        assert tile == 0 or (rows > 128 and tile % 16 == 0 and 64 <= tile <= rules.widest(bf16))
+    assert rules.pair_tile(32, 32, 148, 0, 1, 2048) == 0            # a device that cannot place a pair
