@@ -32,7 +32,7 @@ struct NormArgs {
     uint64_t y_pitch, h_pitch, n_pitch;     // elements
     const void *post_w, *gate, *residual, *pre_w;
     int gate_kind;
-    float y_scale, residual_scale, eps, inv_width;      // y_scale 0 without planes, residual_scale 0 without a residual
+    float y_scale, residual_scale, eps, inv_width;      // y_scale 1 without planes, residual_scale 0 without a residual
     uint32_t rows, width;
     void *h_out, *n_out;
 };
@@ -144,6 +144,11 @@ __device__ __forceinline__ float row_rrms(const float (&v)[E], float inv_width, 
     return rsqrtf(fmaf(ss, inv_width, eps));
 }
 
+// Whether the factors of u that a row shares - y_scale, the token's gate, 1 / rms - may be folded into one, so that u meets them in one
+// multiplication per element. Not where FP32 does not hold their product well (rows of 1e38 and a scale of 1e-6: 1e-44, three bits): then
+// 1 / rms and the gate are applied to the row first. Asked once per row (8,192 x 4,096 BF16 60.8 -> 61.7 us; a branch per vector 73.9).
+__device__ __forceinline__ bool foldable(float product) { return fabsf(product) > 0x1p-32f && fabsf(product) < 0x1p32f; }
+
 // VEC elements as they lie in memory: loads are issued for a whole row before anything waits for one of them.
 template <int VEC, bool F32>
 struct RawVec {
@@ -251,9 +256,15 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) block_norm_kern
                         for (int e = 0; e < VEC; ++e) u[j * VEC + e] += more[z][j].get(e);
         }
         if (rows_at_once < p.rows - row) request(row + rows_at_once);
-        float r1 = p.y_scale;                          // every factor of u that the row shares
+        float r1 = p.y_scale, rrms = 1.0f;             // r1: every factor of u that the row shares
         if (p.gate_kind == kGateToken) r1 *= static_cast<const float*>(p.gate)[row];
-        if (p.post_w) r1 *= row_rrms<E, BLOCK>(u, p.inv_width, p.eps, slots);
+        if (p.post_w) { rrms = row_rrms<E, BLOCK>(u, p.inv_width, p.eps, slots); r1 *= rrms; }
+        if (__builtin_expect(!foldable(r1), 0)) {
+            const float gate = p.gate_kind == kGateToken ? static_cast<const float*>(p.gate)[row] : 1.0f;
+            r1 = p.y_scale;
+#pragma unroll
+            for (int e = 0; e < E; ++e) u[e] = u[e] * rrms * gate;
+        }
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const uint32_t i = (t + j * threads) * VEC;
@@ -337,7 +348,7 @@ __global__ void __launch_bounds__(T, 2048 / T) block_norm_any_kernel(const NormA
     for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x, ++turn) {
         float (*slots)[32] = slots_all[turn & 1];    // the other set may still be read by slower warps of the row before
         const uint64_t yo = row * p.y_pitch, ho = row * p.h_pitch, no = row * p.n_pitch;
-        float r1 = p.y_scale;                          // every factor of u that the row shares
+        float r1 = p.y_scale, rrms = 1.0f;             // r1: every factor of u that the row shares
         if (p.gate_kind == kGateToken) r1 *= static_cast<const float*>(p.gate)[row];
         float ss = 0.0f;
         four([&](uint32_t i, auto full) {
@@ -357,7 +368,12 @@ __global__ void __launch_bounds__(T, 2048 / T) block_norm_any_kernel(const NormA
                 if (kAll || i + e * T < p.width) row_mem[i + e * T] = u[e];
             }
         });
-        if (p.post_w) r1 *= row_rrms_shared(ss, row_mem, p.width, p.inv_width, p.eps, slots);
+        if (p.post_w) { rrms = row_rrms_shared(ss, row_mem, p.width, p.inv_width, p.eps, slots); r1 *= rrms; }
+        if (__builtin_expect(!foldable(r1), 0)) {
+            const float gate = p.gate_kind == kGateToken ? static_cast<const float*>(p.gate)[row] : 1.0f;
+            r1 = p.y_scale;
+            for (uint32_t i = t; i < p.width; i += T) row_mem[i] = row_mem[i] * rrms * gate;
+        }
         ss = 0.0f;
         four([&](uint32_t i, auto full) {
             constexpr bool kAll = decltype(full)::value == 4;

@@ -364,7 +364,7 @@ int m26b_block_norm_dev(const m26b_block_norm_args* args, void* stream, char* er
     a.y_pitch = y_pitch; a.h_pitch = h_pitch; a.n_pitch = n_pitch;
     a.post_w = in.post_w; a.gate = in.gate; a.residual = in.residual; a.pre_w = in.pre_w;
     a.gate_kind = gate_kind;
-    a.y_scale = n_planes ? in.y_scale : 0.0f; a.residual_scale = in.residual ? in.residual_scale : 0.0f; a.eps = in.eps;
+    a.y_scale = n_planes ? in.y_scale : 1.0f; a.residual_scale = in.residual ? in.residual_scale : 0.0f; a.eps = in.eps;
     a.inv_width = 1.0f / float(width);
     a.rows = rows; a.width = width; a.h_out = in.h_out; a.n_out = in.n_out;
     see(in.post_w, w_dtype); see(in.pre_w, w_dtype); see(in.residual, h_dtype); see(in.h_out, h_dtype); see(in.n_out, n_dtype);

@@ -78,3 +78,38 @@ def test_a_wait_that_runs_out_is_reported(torch, rows, n, k, gated):
     got = run(x, rows)
     torch.cuda.synchronize()
     assert int(run.fault) == 0 and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("width", [256, 255, 1000, 4096, 4095, 16384])
+@pytest.mark.parametrize("kind", [0, 1, 2, 3])
+@pytest.mark.parametrize("post", [False, True])
+def test_factors_that_fp32_cannot_hold_as_one(torch, width, kind, post):
+    """Rows of every size FP32 has, with a scale and a gate whose product with the row's 1 / rms lies below its range although the
+    result is ordinary. Every product of two factors is a rounding: 64 u as everywhere."""
+    import mimo26f_afd_b200 as M
+
+    g = D.gen(torch, width + kind)
+    size = torch.tensor([1e38, 1e38, 1e30, 1e20, 1.0, 1e-10, 1e-18], device="cuda")
+    rows = len(size)
+    u = (0.25 + 0.75 * torch.rand(rows, width, device="cuda", generator=g)) * size[:, None]
+    u = torch.where(torch.rand(rows, width, device="cuda", generator=g) < 0.5, -u, u)
+    pw = 0.5 + torch.rand(width, device="cuda", generator=g) if post else None
+    # gates that bring the largest rows down where no norm does
+    weight = torch.tensor([1e-6, 1e-10, 1e-16, 1e-4, 1.0, 1e4, 0.0], device="cuda") * (1.0 if post else 1e-6)
+    gate = None
+    if kind == 1:
+        gate = weight
+    elif kind == 2:
+        gate = 1e-6 + 1e-6 * torch.rand(width, device="cuda", generator=g)
+    elif kind == 3:
+        gate = weight[:, None] * (0.5 + torch.rand(rows, width, device="cuda", generator=g))
+    for ys in (1e-12, 1e-3, -1.0) if post else (1e-25, 1e-12, -1.0):
+        h, n = torch.empty_like(u), torch.empty_like(u)
+        M.block_norm_dev([u], None, rows, width, post_w=pw, gate=gate, gate_kind=kind, y_dtype=1, y_scale=ys, h_out=h, n_out=n, n_dtype=1, eps=1e-6)
+        torch.cuda.synchronize()
+        scale = float(torch.tensor(ys, dtype=torch.float32))
+        want, wn = D.norm_f64([u], None, pw, gate, kind, None, float(torch.tensor(1e-6, dtype=torch.float32)), scale, 1.0)
+        keep = want.abs() >= 2.0**-120                          # below, the result itself runs out of bits
+        assert bool(((h.double() - want).abs() <= 64 * U * want.abs() + 2.0**-149)[keep].all())
+        assert bool((h.double()[~keep].abs() <= 2.0**-119).all())
+        assert bool(((n.double() - wn).abs() <= 128 * U * wn.abs())[keep].all())
