@@ -407,7 +407,7 @@ typedef struct m26b_block_norm_args {
     void* n_out;                /* [rows][width] of n_dtype, n_pitch, or NULL; not both outputs NULL */
     uint64_t y_pitch, h_pitch, n_pitch;
     float y_scale, residual_scale;
-    float eps;                  /* > 0 */
+    float eps;                  /* > 0, a normal number (at least 2^-126, 1.2e-38) */
     uint32_t rows, width;
     int32_t n_planes;           /* 0..8; 0: no block output, then no post_w and no gate */
     int32_t gate_kind;          /* 0 none; 1 one FP32 per token [rows]; 2 one per channel [width], w_dtype; 3 one per element, as a plane */

@@ -345,7 +345,8 @@ int m26b_block_norm_dev(const m26b_block_norm_args* args, void* stream, char* er
         set_msg(err, errlen, "m26b block norm: bad arguments");
         return 1;
     }
-    if (!(in.eps > 0.0f) || in.eps > 3.0e38f) { set_msg(err, errlen, "m26b block norm: eps must be positive"); return 1; }
+    // a square that FP32 holds in part or not at all is off by 2^-150 at most: nothing beside a normal eps, but not beside a subnormal one
+    if (!(in.eps >= 0x1p-126f) || in.eps > 3.0e38f) { set_msg(err, errlen, "m26b block norm: eps must be positive, at least 2^-126"); return 1; }
     const uint64_t y_pitch = in.y_pitch ? in.y_pitch : width, h_pitch = in.h_pitch ? in.h_pitch : width, n_pitch = in.n_pitch ? in.n_pitch : width;
     if (y_pitch < width || h_pitch < width || n_pitch < width) { set_msg(err, errlen, "m26b block norm: a pitch is below the width"); return 1; }
     NormArgs a{};

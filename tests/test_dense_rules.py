@@ -82,3 +82,15 @@ def test_the_chosen_tiles_are_tiles_of_the_kernel(rules):
         tile = rules.pair_tile(2 * int(2 ** rng.uniform(0, 9)), int(2 ** rng.uniform(0, 8)), 148, 148, bf16, rows)
         assert tile == 0 or (rows > 128 and tile % 16 == 0 and 64 <= tile <= rules.widest(bf16))
     assert rules.pair_tile(32, 32, 148, 0, 1, 2048) == 0            # a device that cannot place a pair
+
+
+@pytest.mark.parametrize("eps", [1e-45, 1e-42, 1.17e-38])
+def test_a_subnormal_eps_is_refused(eps):
+    """Rows as small as its root have squares that FP32 cannot hold beside it."""
+    import mimo26f_afd_b200 as M
+
+    p = 0x10000
+    with pytest.raises(M.ExpertError) as e:
+        M.block_norm_dev([p], p, 0, 64, h_out=p, n_out=p, eps=eps)
+    assert e.value.code == 1 and "eps" in e.value.message
+    M.block_norm_dev([p], p, 0, 64, h_out=p, n_out=p, eps=2.0**-126)

@@ -113,3 +113,19 @@ def test_factors_that_fp32_cannot_hold_as_one(torch, width, kind, post):
         assert bool(((h.double() - want).abs() <= 64 * U * want.abs() + 2.0**-149)[keep].all())
         assert bool((h.double()[~keep].abs() <= 2.0**-119).all())
         assert bool(((n.double() - wn).abs() <= 128 * U * wn.abs())[keep].all())
+
+
+@pytest.mark.parametrize("width", [256, 255, 4096, 4095, 16384])
+def test_norms_of_rows_near_the_bottom_of_fp32(torch, width):
+    """Squares that FP32 holds in part or not at all, beside the smallest eps that the norm takes."""
+    import mimo26f_afd_b200 as M
+
+    g = D.gen(torch, width)
+    for eps in (2.0**-126, 1e-36, 1e-30, 1e-20, 1e-6):
+        size = torch.tensor([1e-22, 1e-20, 1e-19, 1e-16, 1e-12, 1.0, 1e30], device="cuda")
+        h = (torch.rand(len(size), width, device="cuda", generator=g) - 0.5) * size[:, None]
+        n = torch.empty_like(h)
+        M.block_norm_dev([], h, len(size), width, n_out=n, n_dtype=1, eps=eps)
+        torch.cuda.synchronize()
+        _, want = D.norm_f64([], h, None, None, 0, None, float(torch.tensor(eps, dtype=torch.float32)), 1.0, 1.0)
+        assert bool(((n.double() - want).abs() <= 64 * U * want.abs() + 2.0**-149).all()), eps
