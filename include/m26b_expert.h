@@ -359,7 +359,8 @@ int m26b_plan_static(const int32_t* ids, const float* weights, uint32_t rows, in
  *              FP32. Only y's n columns of `rows` rows are written. One token to a prefill batch (passes of 8,192; at most
  *              2^31 - 1 rows); 0 rows is no work. BF16 activations are not quantised: a K32 block enters the product as two E4M3
  *              pieces that equal it exactly, save for elements below 2^-13 of the block's largest, which carry an error of
- *              at most 2^-21 of that largest. Products accumulate in FP32. A row with an infinity, a NaN (or, for E4M3, a NaN
+ *              at most 2^-21 of that largest. Products accumulate in FP32; a sum beyond FP32 is infinite, or NaN. The activation is within
+ *              2^-19 of itself (relative) whatever its argument. A row with an infinity, a NaN (or, for E4M3, a NaN
  *              code or scale byte 255) in it is NaN in all its outputs. A row's result does not change with the other rows'
  *              values. Nothing is allocated, nothing is synchronised, and a call can be captured into a graph; the handle
  *              must stay alive until the work is done, the argument record is read before the call returns. Enqueued on

@@ -254,12 +254,19 @@ __device__ __forceinline__ bool acc_wait(uint64_t* bar, uint32_t parity, volatil
     return false;
 }
 
-__device__ __forceinline__ float silu_gate(float g, float u) {
-    // g / (1 + e^-g) * u without a positive exponential; infinities of g give +inf * u and -0 * u
-    const float e = __expf(-fabsf(g));
-    const float s = __fdividef(g >= 0.0f ? 1.0f : e, 1.0f + e);
-    return g * s * u;
+// g / (1 + e^-g) * u without a positive exponential, within 2^-19 of itself for every g. expf and not the approximation, whose error grows
+// with |g| (2^-18 at -60). `near`: g >= -64, where e^g is a normal number; an infinite g gives inf * u. `far`: any g; e^(g / 2) is met
+// twice, so that g e^g u is whole where e^g alone has left FP32. Below -512 nothing is left whatever u is: -inf gives -0 * u.
+constexpr float kSiluFar = -64.0f;
+__device__ __forceinline__ float silu_near(float g, float u) {
+    const float e = expf(-fabsf(g));
+    return g * __fdividef(g >= 0.0f ? 1.0f : e, 1.0f + e) * u;
 }
+__device__ __forceinline__ float silu_far(float g, float u) {
+    const float c = g < -512.0f ? -512.0f : g, h = expf(-0.5f * fabsf(c)), d = c >= 0.0f ? 1.0f : h;
+    return __fdividef(c * d, fmaf(h, h, 1.0f)) * u * d;
+}
+__device__ __forceinline__ float silu_gate(float g, float u) { return g < kSiluFar ? silu_far(g, u) : silu_near(g, u); }
 __device__ __forceinline__ void store_y(const LinearArgs& p, uint32_t token, uint32_t col, float v) {
     const uint64_t at = uint64_t(token) * p.y_pitch + col;
     if (p.y_f32) static_cast<float*>(p.y)[at] = v;
@@ -271,12 +278,26 @@ template <bool GATED>
 __device__ __forceinline__ void store_columns(const LinearArgs& p, const uint32_t (&r)[16], uint32_t token, uint32_t end, uint32_t feat, int lane) {
     if constexpr (GATED) {
         const bool upper = lane >= 16;
+        float g[8], u[8], low = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-            const float other = __uint_as_float(__shfl_xor_sync(0xffffffffu, upper ? r[j] : r[j + 1], 16));
-            const float mine = __uint_as_float(upper ? r[j + 1] : r[j]);
-            const uint32_t t = token + j + (upper ? 1 : 0);
-            if (t < end && feat < p.n) store_y(p, t, feat, upper ? silu_gate(other, mine) : silu_gate(mine, other));
+        for (int j = 0; j < 8; ++j) {
+            const float other = __uint_as_float(__shfl_xor_sync(0xffffffffu, upper ? r[2 * j] : r[2 * j + 1], 16));
+            const float mine = __uint_as_float(upper ? r[2 * j + 1] : r[2 * j]);
+            g[j] = upper ? other : mine;
+            u[j] = upper ? mine : other;
+            low = fminf(low, g[j]);
+        }
+        if (__builtin_expect(low < kSiluFar, 0)) {       // asked once for the eight: hardly any gate is
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = silu_gate(g[j], u[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = silu_near(g[j], u[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t t = token + 2 * j + (upper ? 1 : 0);
+            if (t < end && feat < p.n) store_y(p, t, feat, u[j]);
         }
     } else {
 #pragma unroll

@@ -129,3 +129,79 @@ def test_norms_of_rows_near_the_bottom_of_fp32(torch, width):
         torch.cuda.synchronize()
         _, want = D.norm_f64([], h, None, None, 0, None, float(torch.tensor(eps, dtype=torch.float32)), 1.0, 1.0)
         assert bool(((n.double() - want).abs() <= 64 * U * want.abs() + 2.0**-149).all()), eps
+
+
+@pytest.mark.parametrize("rows,n", [(24, 64), (100, 4100), (130, 64), (2000, 9600)])
+def test_the_activation_over_the_whole_range_of_its_argument(torch, rows, n):
+    """One gate weight and one up weight per feature, both 1: y = silu(x[0]) * x[32]. Two exponentials of half the argument (2 units each, met
+    twice), a quotient (2 units) and three products: within 2^-19 of the result for every gate, as far as FP32 reaches."""
+    import mimo26f_afd_b200 as M
+
+    k = 64
+    weight = torch.zeros(n, k // 2, dtype=torch.uint8, device="cuda")
+    gw, uw = weight.clone(), weight.clone()
+    gw[:, 0], uw[:, 16] = 2, 2
+    s = torch.full((n, k // 32), 127, dtype=torch.uint8, device="cuda")
+    g = D.gen(torch, rows)
+    size = torch.exp2(torch.rand(rows, device="cuda", generator=g) * 20 - 10)
+    size[:12] = torch.tensor([60.0, 70, 80, 88, 90, 95, 100, 103.5, 110, 140, 170, 3e38], device="cuda")
+    sign = torch.where(torch.arange(rows, device="cuda") % 3 == 0, 1.0, -1.0)
+    sign[:12] = -1.0
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = size * sign
+    for up in (1.0, -1e30, 1e38):
+        x[:, 32] = up
+        run = D.Runner(torch, M.Linear.gated(gw, s, uw, s, n, k), rows)
+        a = x[:, 0].double()
+        want = (a * torch.sigmoid(a) * x[:, 32].double())[:, None].expand(rows, n)
+        keep = want.abs() < 3.4e38
+        y = run(x, rows)
+        torch.cuda.synchronize()
+        off = (y.double() - want).abs()
+        assert bool((off <= 2.0**-19 * want.abs() + 2.0**-126 * 2.0**-19)[keep].all()), float((off / want.abs().clamp_min(2.0**-126))[keep].max()) * 2**19
+        assert torch.equal(y[~keep], want.float()[~keep])
+
+
+@pytest.mark.parametrize("rows", [5, 130])
+@pytest.mark.parametrize("quantised", [False, True])
+def test_gate_sums_beyond_fp32(torch, rows, quantised):
+    """-inf gives -0 * u, as every gate below some -200 does; +inf gives inf * u."""
+    import mimo26f_afd_b200 as M
+
+    n, k = 64, 64
+    gw, uw = (torch.zeros(n, k // 2, dtype=torch.uint8, device="cuda") for _ in range(2))
+    gw[:, 0], uw[:, 16] = 7, 2
+    gs, us = (torch.full((n, k // 32), b, dtype=torch.uint8, device="cuda") for b in (154, 127))
+    run = D.Runner(torch, M.Linear.gated(gw, gs, uw, us, n, k), rows)
+    if quantised:                                                # gates of 6 * 2^27 * 448 * 2^100
+        q = torch.zeros(rows, k, dtype=torch.uint8, device="cuda")
+        q[:, 32] = 0x44                                          # 3
+        q[0::2, 0], q[1::2, 0] = 0xfe, 0x7e
+        xs = torch.full((rows, k // 32), 127, dtype=torch.uint8, device="cuda")
+        xs[:, 0] = 227
+        y = run(q, rows, x_scales=xs)
+    else:                                                        # gates of 6 * 2^27 * 1e30 = 8e38
+        x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+        x[:, 32] = 3.0
+        x[0::2, 0], x[1::2, 0] = -1e30, 1e30
+        y = run(x, rows)
+    torch.cuda.synchronize()
+    assert bool((y[0::2] == 0.0).all()) and bool((y[1::2] == float("inf")).all())
+
+
+def test_far_gates_of_other_rows_change_nothing(torch):
+    """The exact form for far gates is a choice per element: not of the rows beside it, nor of what pads the tile."""
+    import mimo26f_afd_b200 as M
+
+    n, k, rows = 320, 256, 37
+    g = D.gen(torch, 21)
+    gw, gs = D.make_weights(torch, n, k, g)
+    uw, us = D.make_weights(torch, n, k, g)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(torch.bfloat16)
+    run = D.Runner(torch, M.Linear.gated(gw, gs, uw, us, n, k), rows)
+    want = run(x, rows).clone()
+    x2 = x.clone()
+    x2[1::2] *= 1000.0
+    got = run(x2, rows)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0::2], want[0::2])
