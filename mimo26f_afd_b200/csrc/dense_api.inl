@@ -11,7 +11,7 @@ struct m26b_linear {
     bool gated = false;
     int device = 0, sms = 0;
     uint32_t tiles = 0;                         // 128-row tiles of the image (even)
-    int khz = 0;                                // nominal SM clock
+    m26b::LinearShape shape{};                  // the same for the host's rules, with what the device can place
     long long wait_cycles = kWaitCycles;        // bound of the epilogues' wait for their accumulators
     CUtensorMap map_w, map_sf;
 };
@@ -22,6 +22,33 @@ static_assert(linear_widest_pair_tile(true) == LinearPairTile<2>::kTokens && lin
               kChunkK == 128 && kScaleBlockBytes == 512, "linear_rules.h knows the kernels' widest tiles, a chunk and a scale block");
 constexpr uint32_t kLinearMaxDim = 1u << 20;
 constexpr uint32_t kDenseMaxRows = 0x7fffffffu;
+
+// Asked about in place of the product's kernels, never launched: for a kernel that allocates tensor memory the occupancy calls answer one CTA
+// per SM whatever it needs (256 CTAs of 4,096 x 16,384 for one token, two on most SMs: 10.3 us; the 128 that the calls grant: 15.1).
+__global__ void linear_room_kernel() {}
+
+// CTAs that run at once in clusters of 1 << log_size (0 if the device cannot place one): GPCs hold whole clusters, and not all have the same SMs.
+template <int B_ROWS>
+cudaError_t linear_room(int sms, uint32_t (&room)[4]) {
+    using T = LinearTile<B_ROWS, 2>;
+    const int smem = int(sizeof(LinearSmem<B_ROWS, 2>)) + 1024;
+    const cudaError_t e = cudaFuncSetAttribute(linear_room_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    room[0] = uint32_t(sms * T::kCtasPerSm);
+    for (uint32_t log_size = 1; log_size < 4; ++log_size) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(room[0] >> log_size << log_size); cfg.blockDim = dim3(T::kThreads); cfg.dynamicSmemBytes = size_t(smem);
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = 1u << log_size; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+        cfg.attrs = &at; cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, linear_room_kernel, &cfg) != cudaSuccess) { clusters = 0; cudaGetLastError(); }
+        const uint32_t ctas = uint32_t(clusters) << log_size;
+        room[log_size] = ctas < room[0] ? ctas : room[0];
+    }
+    return cudaSuccess;
+}
 
 int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool gated, uint32_t n, uint32_t k, m26b_linear** out, char* err,
                size_t errlen) {
@@ -45,9 +72,10 @@ int linear_new(const uint8_t* const (&w)[2], const uint8_t* const (&s)[2], bool 
     };
     cudaError_t e = cudaGetDevice(&L->device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&L->sms, cudaDevAttrMultiProcessorCount, L->device);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&L->khz, cudaDevAttrClockRate, L->device);
     if (e != cudaSuccess) return fail("m26b linear device", e);
-    if (L->khz <= 0) L->khz = 1965000;
+    L->shape.tiles = L->tiles; L->shape.chunks = uint32_t(chunks); L->shape.sms = uint32_t(L->sms);
+    if ((e = linear_room<128>(L->sms, L->shape.room[0])) != cudaSuccess || (e = linear_room<16>(L->sms, L->shape.room[1])) != cudaSuccess)
+        return fail("m26b linear occupancy", e);
     if ((e = cudaDeviceSynchronize()) != cudaSuccess) return fail("m26b linear sync", e);      // the source may come from any stream
     void* mem = nullptr;
     if ((e = cudaMalloc(&mem, w_bytes)) != cudaSuccess) return fail("m26b linear weights alloc", e);
@@ -81,7 +109,7 @@ cudaError_t launch_linear(const m26b_linear* L, const TokenMaps& mx, const Linea
         opted.fetch_or(bit, std::memory_order_relaxed);
     }
     const uint32_t feats = GATED ? 64 : kTileM, tiles = (a.n + feats - 1) / feats, tok_tiles = (a.rows + B_ROWS - 1) / B_ROWS;
-    const uint32_t log_split = linear_log_split(uint64_t(tiles) * tok_tiles, uint64_t(L->sms), T::kCtasPerSm, a.chunks);
+    const uint32_t log_split = linear_log_split(L->shape, uint64_t(tiles) * tok_tiles, T::kCtasPerSm, a.chunks);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(tiles << log_split, tok_tiles); cfg.blockDim = dim3(T::kThreads); cfg.dynamicSmemBytes = size_t(smem); cfg.stream = st;
     cudaLaunchAttribute at[2]{};
@@ -154,9 +182,8 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
                        L->wait_cycles};
     TokenMaps mx{};
     cudaError_t e;
-    const LinearShape shape{L->tiles, L->k_pad / kChunkK, uint32_t(L->sms)};
-    const uint32_t pair_tile = rows <= 128 ? 0 : linear_pair_tile(shape, linear_pair_ctas(L, bf16), bf16, rows), tile = pair_tile ? pair_tile : rows <= 64 ? 64u : 128u;
-    if (vec && !pair_tile && linear_direct(shape, bf16, rows)) {
+    const uint32_t pair_tile = rows <= 128 ? 0 : linear_pair_tile(L->shape, linear_pair_ctas(L, bf16), bf16, rows), tile = pair_tile ? pair_tile : rows <= 64 ? 64u : 128u;
+    if (vec && !pair_tile && linear_direct(L->shape, bf16, rows)) {
         if (rows <= 16) e = launch_linear_tile<16, true>(L, bf16, mx, a, st);
         else if (rows <= 32) e = launch_linear_tile<32, true>(L, bf16, mx, a, st);
         else if (rows <= 64) e = launch_linear_tile<64, true>(L, bf16, mx, a, st);
@@ -199,30 +226,40 @@ int linear_pass(const m26b_linear* L, const void* x, bool bf16, const uint8_t* x
     return 0;
 }
 
+// SMs of a device, 0 if it cannot be asked.
+uint32_t device_sms(int dev) {
+    static std::atomic<uint32_t> known[64]{};                          // by device of this process
+    uint32_t sms = known[dev & 63].load(std::memory_order_relaxed);
+    if (!sms) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); return 0; }
+        known[dev & 63].store(sms = uint32_t(n), std::memory_order_relaxed);
+    }
+    return sms;
+}
 // Rows are strided over by as many CTAs as the GPU holds at once.
 template <int VEC, int PER, int THREADS, bool Y32, bool H32, bool GATE_ELEM>
-cudaError_t launch_norm_kernel(const NormArgs& a, cudaStream_t st) {
+cudaError_t launch_norm_kernel(const NormArgs& a, int dev, cudaStream_t st) {
     const auto kernel = block_norm_kernel<VEC, PER, THREADS, Y32, H32, GATE_ELEM>;
     constexpr uint32_t block = THREADS == 32 ? 128 : THREADS;
-    static std::atomic<uint32_t> known{0};                             // CTAs the device holds: the same for every GPU of the box
-    uint32_t room = known.load(std::memory_order_relaxed);
+    static std::atomic<uint32_t> known[64]{};                          // CTAs the device holds, by device of this process
+    uint32_t room = known[dev & 63].load(std::memory_order_relaxed);
     if (!room) {
-        int dev = 0, sms = 0, per_sm = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, int(block), 0);
-        if (e != cudaSuccess || per_sm < 1) return e != cudaSuccess ? e : cudaErrorLaunchOutOfResources;
-        room = uint32_t(sms * per_sm);
-        known.store(room, std::memory_order_relaxed);
+        int per_sm = 0;
+        const uint32_t sms = device_sms(dev);
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, int(block), 0);
+        if (e != cudaSuccess || per_sm < 1 || !sms) return e != cudaSuccess ? e : cudaErrorLaunchOutOfResources;
+        room = sms * uint32_t(per_sm);
+        known[dev & 63].store(room, std::memory_order_relaxed);
     }
     const uint32_t need = THREADS == 32 ? (a.rows + 3) / 4 : a.rows;
     return launch_dependent(kernel, need < room ? need : room, block, 0, st, a);
 }
 template <int VEC, int PER, int THREADS>
-cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
+cudaError_t launch_norm(const NormArgs& a, int dev, cudaStream_t st) {
     const auto typed = [&](auto y32, auto h32) {
-        if (a.gate_kind == kGateElement) return launch_norm_kernel<VEC, PER, THREADS, y32.value, h32.value, true>(a, st);
-        return launch_norm_kernel<VEC, PER, THREADS, y32.value, h32.value, false>(a, st);
+        if (a.gate_kind == kGateElement) return launch_norm_kernel<VEC, PER, THREADS, y32.value, h32.value, true>(a, dev, st);
+        return launch_norm_kernel<VEC, PER, THREADS, y32.value, h32.value, false>(a, dev, st);
     };
     constexpr std::true_type yes{};
     constexpr std::false_type no{};
@@ -232,41 +269,38 @@ cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
 // Threads and vectors per thread by width: a row's CTA is as small as its registers allow (8,192 x 4,096: 62 us with two vectors of
 // eight in each of 256 threads, 87 with one in 512, 72 with four in 128), since what a row costs beyond its bytes is two
 // reductions over its threads. Wider rows than 8,192 do not fit the registers of a CTA and take block_norm_any_kernel.
-cudaError_t launch_norm_vec8(const NormArgs& a, cudaStream_t st) {
-    if (a.width <= 512) return launch_norm<8, 2, 32>(a, st);
-    if (a.width <= 1024) return launch_norm<8, 2, 64>(a, st);
-    if (a.width <= 2048) return launch_norm<8, 2, 128>(a, st);
-    if (a.width <= 4096) return launch_norm<8, 2, 256>(a, st);
-    return launch_norm<8, 2, 512>(a, st);
+cudaError_t launch_norm_vec8(const NormArgs& a, int dev, cudaStream_t st) {
+    if (a.width <= 512) return launch_norm<8, 2, 32>(a, dev, st);
+    if (a.width <= 1024) return launch_norm<8, 2, 64>(a, dev, st);
+    if (a.width <= 2048) return launch_norm<8, 2, 128>(a, dev, st);
+    if (a.width <= 4096) return launch_norm<8, 2, 256>(a, dev, st);
+    return launch_norm<8, 2, 512>(a, dev, st);
 }
-cudaError_t launch_norm_vec4(const NormArgs& a, cudaStream_t st) {
-    if (a.width <= 1024) return launch_norm<4, 4, 64>(a, st);
-    if (a.width <= 4096) return launch_norm<4, 4, 256>(a, st);
-    return launch_norm<4, 4, 512>(a, st);
+cudaError_t launch_norm_vec4(const NormArgs& a, int dev, cudaStream_t st) {
+    if (a.width <= 1024) return launch_norm<4, 4, 64>(a, dev, st);
+    if (a.width <= 4096) return launch_norm<4, 4, 256>(a, dev, st);
+    return launch_norm<4, 4, 512>(a, dev, st);
 }
 template <uint32_t T, bool Y32, bool H32>
-cudaError_t launch_norm_any(const NormArgs& a, cudaStream_t st) {
+cudaError_t launch_norm_any(const NormArgs& a, int dev, cudaStream_t st) {
     const auto kernel = block_norm_any_kernel<T, Y32, H32>;
     const size_t smem = size_t(a.width) * 4;
     static std::atomic<uint64_t> opted{0};                             // one flag bit per device of this process
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
     const uint64_t bit = 1ull << (dev & 63);
     if (!(opted.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kNormMaxWidth) * 4);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kNormMaxWidth) * 4);
         if (e != cudaSuccess) return e;
         opted.fetch_or(bit, std::memory_order_relaxed);
     }
     return launch_dependent(kernel, a.rows, T, smem, st, a);
 }
 template <bool Y32, bool H32>
-cudaError_t launch_norm_any_width(const NormArgs& a, cudaStream_t st) {
-    // many rows: CTAs so small that eight of them share an SM (8,192 x 4,095: 101 us, 178 with 1,024 threads); few rows: the threads
-    // of one SM on one row (1 x 4,095: 4.4 us, 7.0 with 256)
-    if (a.width <= 512) return launch_norm_any<64, Y32, H32>(a, st);
-    if (a.width <= 1024 || (a.width <= 8192 && a.rows > 296)) return launch_norm_any<256, Y32, H32>(a, st);
-    return launch_norm_any<1024, Y32, H32>(a, st);
+cudaError_t launch_norm_any_width(const NormArgs& a, int dev, cudaStream_t st) {
+    // more rows than large CTAs fit the device (two per SM): CTAs so small that eight of them share an SM (8,192 x 4,095: 101 us, 178 with
+    // 1,024 threads); fewer: the threads of one SM on one row (1 x 4,095: 4.4 us, 7.0 with 256)
+    if (a.width <= 512) return launch_norm_any<64, Y32, H32>(a, dev, st);
+    if (a.width <= 1024 || (a.width <= 8192 && a.rows > 2 * device_sms(dev))) return launch_norm_any<256, Y32, H32>(a, dev, st);
+    return launch_norm_any<1024, Y32, H32>(a, dev, st);
 }
 
 }  // namespace
@@ -290,7 +324,9 @@ void m26b_linear_free(m26b_linear* l) {
 }
 int m26b_linear_set_wait_us(m26b_linear* l, uint32_t us) {
     if (!l || !us) return 1;
-    l->wait_cycles = (long long)us * l->khz / 1000;
+    int khz = 0;                                // nominal SM clock; the call takes half a millisecond, so not in every linear_new
+    if (cudaDeviceGetAttribute(&khz, cudaDevAttrClockRate, l->device) != cudaSuccess || khz <= 0) { cudaGetLastError(); khz = 1965000; }
+    l->wait_cycles = (long long)us * khz / 1000;
     return 0;
 }
 uint64_t m26b_linear_workspace_bytes(const m26b_linear* l, uint32_t rows) {
@@ -375,11 +411,13 @@ int m26b_block_norm_dev(const m26b_block_norm_args* args, void* stream, char* er
     if (!rows) return 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const uint64_t pitches = (n_planes ? y_pitch : 0) | (in.residual || in.h_out ? h_pitch : 0) | (in.n_out ? n_pitch : 0);
-    cudaError_t e;
-    if (!vec8 && (width | pitches) % 8 == 0 && width <= 8192) e = launch_norm_vec8(a, st);
-    else if (!vec4 && pitches % 4 == 0 && width <= 8192) e = launch_norm_vec4(a, st);
-    else if (y_dtype) e = h_dtype ? launch_norm_any_width<true, true>(a, st) : launch_norm_any_width<true, false>(a, st);
-    else e = h_dtype ? launch_norm_any_width<false, true>(a, st) : launch_norm_any_width<false, false>(a, st);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) { set_err(err, errlen, "m26b block norm device", e); return 2; }
+    if (!vec8 && (width | pitches) % 8 == 0 && width <= 8192) e = launch_norm_vec8(a, dev, st);
+    else if (!vec4 && pitches % 4 == 0 && width <= 8192) e = launch_norm_vec4(a, dev, st);
+    else if (y_dtype) e = h_dtype ? launch_norm_any_width<true, true>(a, dev, st) : launch_norm_any_width<true, false>(a, dev, st);
+    else e = h_dtype ? launch_norm_any_width<false, true>(a, dev, st) : launch_norm_any_width<false, false>(a, dev, st);
     if (e != cudaSuccess) { cudaGetLastError(); set_err(err, errlen, "m26b block norm launch", e); return 2; }
     return 0;
 }

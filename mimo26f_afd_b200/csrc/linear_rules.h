@@ -13,6 +13,7 @@ constexpr uint32_t linear_widest_pair_tile(bool bf16) { return bf16 ? 224 : 256;
 struct LinearShape {
     uint32_t tiles, chunks;     // 128-row tiles of the weight image, 128-wide chunks of K
     uint32_t sms;
+    uint32_t room[2][4];        // [CTAs per SM - 1][log2 of the cluster size]: CTAs that run at once, as the device says
 };
 
 inline uint32_t linear_rows_cap(uint32_t rows) { return ((rows < kLinearPassRows ? rows : kLinearPassRows) + 15) & ~15u; }
@@ -33,13 +34,12 @@ inline uint64_t linear_workspace(uint32_t k_pad, uint32_t rows) {
 }
 
 // log2 of the CTAs that share a weight tile's K (a cluster): doubled while the clusters still run at once and each CTA keeps at least
-// two chunks. A GPC holds whole clusters only: of the 148 SMs, 33 clusters of four run at once and fifteen of eight with one CTA per SM
-// (66 and 32 with two), and what is left would run as a second round (100 tokens, 2,048 x 2,048, sixteen clusters of eight: 15.2 us,
-// of four: 8.3). Powers of two: the divisions that other sizes need cost 0.3 us, more than they gain.
-inline uint32_t linear_log_split(uint64_t ctas, uint64_t sms, uint32_t per_sm, uint32_t chunks) {
-    const uint64_t slots = sms * per_sm, room[4] = {slots, slots, slots * 892 / 1000, slots * (per_sm == 2 ? 865 : 811) / 1000};
+// two chunks. A GPC holds whole clusters only, so that fewer of them run at once than SMs over cluster size (of the 148 SMs here 33 clusters of
+// four and fifteen of eight with one CTA per SM, 71 and 33 with two), and what is left would run as a second round (100 tokens, 2,048 x
+// 2,048, sixteen clusters of eight: 15.2 us, of four: 8.3; 16 tokens, 4,224 x 16,384: 11.5 and 16.6). Powers of two: the divisions that other sizes need cost 0.3 us, more than they gain.
+inline uint32_t linear_log_split(const LinearShape& L, uint64_t ctas, uint32_t per_sm, uint32_t chunks) {
     uint32_t log_split = 0;
-    while (log_split < 3 && (ctas << (log_split + 1)) <= room[log_split + 1] && chunks >= 4u << log_split) ++log_split;
+    while (log_split < 3 && (ctas << (log_split + 1)) <= L.room[per_sm - 1][log_split + 1] && chunks >= 4u << log_split) ++log_split;
     return log_split;
 }
 // Whether a request that single CTAs run converts its activations (rows on vector boundaries) inside the product's kernel. Up to 32 tokens
@@ -49,7 +49,7 @@ inline uint32_t linear_log_split(uint64_t ctas, uint64_t sms, uint32_t per_sm, u
 inline bool linear_direct(const LinearShape& L, bool bf16, uint32_t rows) {
     if (rows <= (bf16 ? 32u : 64u)) return true;
     const uint64_t ctas = uint64_t(L.tiles) * ((rows + 127) / 128);
-    const uint32_t per_cta = L.chunks >> linear_log_split(ctas, L.sms, 1, L.chunks);
+    const uint32_t per_cta = L.chunks >> linear_log_split(L, ctas, 1, L.chunks);
     return ctas <= L.sms && per_cta * (rows < 128 ? rows : 128) <= (bf16 ? 256u : 512u);
 }
 // Token tile of the CTA-pair kernel (`ctas`: how many of its CTAs run at once) for a request, or 0 if single CTAs (which can split K)
@@ -73,7 +73,7 @@ inline uint32_t linear_pair_tile(const LinearShape& L, uint32_t ctas, bool bf16,
     for (uint32_t tile = widest - 16; tile >= kLinearMinPairTile; tile -= 16)
         if (pair_cost(tile) < cost) { best = tile; cost = pair_cost(tile); }
     const uint64_t single = uint64_t(L.tiles) * ((rows + 127) / 128), sms = L.sms;
-    const uint32_t log_split = linear_log_split(single, sms, 1, L.chunks);
+    const uint32_t log_split = linear_log_split(L, single, 1, L.chunks);
     const uint64_t single_cost = ((single << log_split) + sms - 1) / sms * ((L.chunks >> log_split) * (bf16 ? 768 : 512) + 4000);
     return pair_cost(best) < single_cost ? best : 0;
 }

@@ -32,14 +32,24 @@ using namespace m26b;
 extern "C" {
 uint64_t workspace(uint32_t k_pad, uint32_t rows) { return linear_workspace(k_pad, rows); }
 uint64_t blocks(uint32_t rows, uint32_t tile, uint32_t pieces) { return linear_scale_blocks(rows, tile, pieces); }
-uint32_t pair_tile(uint32_t tiles, uint32_t chunks, uint32_t sms, uint32_t ctas, int bf16, uint32_t rows) { return linear_pair_tile({tiles, chunks, sms}, ctas, bf16, rows); }
+static LinearShape shape(uint32_t tiles, uint32_t chunks, const uint32_t* place) {          // place: SMs, room[2][4]
+    LinearShape s{tiles, chunks, place[0], {}};
+    for (int i = 0; i < 8; ++i) s.room[i / 4][i % 4] = place[1 + i];
+    return s;
+}
+uint32_t pair_tile(uint32_t tiles, uint32_t chunks, const uint32_t* place, uint32_t ctas, int bf16, uint32_t rows) { return linear_pair_tile(shape(tiles, chunks, place), ctas, bf16, rows); }
+uint32_t log_split(uint32_t tiles, uint32_t chunks, const uint32_t* place, uint64_t ctas, uint32_t per_sm) { return linear_log_split(shape(tiles, chunks, place), ctas, per_sm, chunks); }
+uint32_t direct(uint32_t tiles, uint32_t chunks, const uint32_t* place, int bf16, uint32_t rows) { return linear_direct(shape(tiles, chunks, place), bf16, rows); }
 uint32_t widest(int bf16) { return linear_widest_pair_tile(bf16); }
 }
 ''')
     subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", f"{ROOT}/mimo26f_afd_b200/csrc", "-o", str(d / "rules.so"), str(d / "rules.cpp")], check=True)
     lib = C.CDLL(str(d / "rules.so"))
     lib.workspace.restype = lib.blocks.restype = C.c_uint64
-    lib.pair_tile.restype = lib.widest.restype = C.c_uint32
+    for f in (lib.pair_tile, lib.widest, lib.log_split, lib.direct):
+        f.restype = C.c_uint32
+    lib.log_split.argtypes = [C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint64, C.c_uint32]
+    lib.b200 = (C.c_uint32 * 9)(148, 148, 148, 132, 120, 296, 296, 284, 264)       # as a B200 answers
     return lib
 
 
@@ -79,9 +89,9 @@ def test_the_chosen_tiles_are_tiles_of_the_kernel(rules):
     rng = random.Random(7)
     for _ in range(20000):
         bf16, rows = rng.random() < 0.5, int(2 ** rng.uniform(0, 13))
-        tile = rules.pair_tile(2 * int(2 ** rng.uniform(0, 9)), int(2 ** rng.uniform(0, 8)), 148, 148, bf16, rows)
+        tile = rules.pair_tile(2 * int(2 ** rng.uniform(0, 9)), int(2 ** rng.uniform(0, 8)), rules.b200, 148, bf16, rows)
         assert tile == 0 or (rows > 128 and tile % 16 == 0 and 64 <= tile <= rules.widest(bf16))
-    assert rules.pair_tile(32, 32, 148, 0, 1, 2048) == 0            # a device that cannot place a pair
+    assert rules.pair_tile(32, 32, rules.b200, 0, 1, 2048) == 0            # a device that cannot place a pair
 
 
 @pytest.mark.parametrize("eps", [1e-45, 1e-42, 1.17e-38])
@@ -94,3 +104,20 @@ def test_a_subnormal_eps_is_refused(eps):
         M.block_norm_dev([p], p, 0, 64, h_out=p, n_out=p, eps=eps)
     assert e.value.code == 1 and "eps" in e.value.message
     M.block_norm_dev([p], p, 0, 64, h_out=p, n_out=p, eps=2.0**-126)
+
+
+def test_a_k_split_is_as_wide_as_the_device_places(rules):
+    """No more clusters than run at once, whatever the device's GPCs hold; at least two chunks per CTA."""
+    import ctypes as C
+
+    places = [rules.b200, (C.c_uint32 * 9)(132, 132, 132, 128, 112, 264, 264, 256, 224), (C.c_uint32 * 9)(148, 148, 146, 120, 96, 296, 292, 240, 192),
+              (C.c_uint32 * 9)(16, 16, 16, 0, 0, 32, 32, 0, 0)]
+    for place in places:
+        for per_sm in (1, 2):
+            room = place[1 + 4 * (per_sm - 1):5 + 4 * (per_sm - 1)]
+            for ctas in (1, 2, 7, 16, 32, 33, 60, 66, 74, 100, 148, 149, 300, 5000):
+                for chunks in (1, 2, 3, 4, 7, 8, 16, 100):
+                    s = rules.log_split(2, chunks, place, ctas, per_sm)
+                    fits = [(ctas << i) <= room[i] and chunks >> i >= 2 for i in (1, 2, 3)]
+                    assert s == next((i for i, ok in enumerate(fits) if not ok), 3), (list(place), per_sm, ctas, chunks)
+    assert rules.log_split(2, 16, places[0], 16, 1) == 2 and rules.log_split(2, 16, places[0], 15, 1) == 3      # fifteen clusters of eight
