@@ -47,6 +47,11 @@ def _addr(x) -> int:
         return _ptr(x)
 
 
+def _any_addr(x):
+    """The address of a buffer of no rows: an empty tensor has none, and any stands for it, since nothing is read or written."""
+    return x if x is None or type(x) is int else _addr(x) or 1 << 20
+
+
 class Linear:
     """One prepared MXFP4 matrix (``new``: y = x W^T) or gated pair (``gated``: silu(x Wg^T) * (x Wu^T)) on the current
     device. Weights ``w`` u8 [n, k/2], scales ``s`` u8 [n, k/32]; the sources may be freed afterwards."""
@@ -118,8 +123,12 @@ def block_norm_dev(planes, residual, rows: int, width: int, *, post_w=None, gate
                    w_dtype: int = 1, eps: float = 1e-6, h_out=None, n_out=None, n_dtype: int = 0, n_pitch: int = 0, stream=None) -> None:
     """u = sum of ``planes`` in order, normed with ``post_w`` if given; h = residual_scale * residual + y_scale * gate * u into
     ``h_out``; n = the RMS norm of h (times ``pre_w``) into ``n_out``. dtypes 0 = BF16, 1 = FP32; pitches in elements, 0 =
-    dense rows; ``planes`` a sequence of up to eight device buffers (empty: norm of the residual alone)."""
+    dense rows; ``planes`` a sequence of up to eight device buffers (empty: norm of the residual alone). No rows are no work; the
+    other arguments are checked all the same, and empty tensors are fine."""
     n = len(planes)
+    if not rows:
+        planes = [_any_addr(p) for p in planes]
+        gate, residual, h_out, n_out = _any_addr(gate), _any_addr(residual), _any_addr(h_out), _any_addr(n_out)
     if n > 8:
         raise ExpertError(1, "m26b block norm: bad arguments")
     try:

@@ -121,3 +121,24 @@ def test_a_k_split_is_as_wide_as_the_device_places(rules):
                     fits = [(ctas << i) <= room[i] and chunks >> i >= 2 for i in (1, 2, 3)]
                     assert s == next((i for i, ok in enumerate(fits) if not ok), 3), (list(place), per_sm, ctas, chunks)
     assert rules.log_split(2, 16, places[0], 16, 1) == 2 and rules.log_split(2, 16, places[0], 15, 1) == 3      # fifteen clusters of eight
+
+
+def test_no_rows_of_empty_tensors_are_no_work():
+    """A rank without tokens has empty tensors, whose address is 0; a missing argument is refused as with rows."""
+    import torch
+
+    import mimo26f_afd_b200 as M
+
+    e = torch.empty(0, 64)
+    assert e.data_ptr() == 0
+    w = torch.ones(64)
+    M.block_norm_dev([e], e, 0, 64, h_out=e, n_out=e)
+    M.block_norm_dev([e, e, e], e, 0, 64, post_w=w, gate=torch.empty(0), gate_kind=M.GATE_TOKEN, pre_w=w, h_out=e, n_out=e)
+    M.block_norm_dev([e], None, 0, 64, gate=e, gate_kind=M.GATE_ELEMENT, n_out=e)
+    M.block_norm_dev([], e, 0, 64, n_out=e)
+    for kw in (dict(residual=None, planes=[]), dict(h_out=None, n_out=None), dict(gate_kind=M.GATE_TOKEN), dict(planes=[e, None]), dict(width=0)):
+        a = dict(planes=[e], residual=e, rows=0, width=64, h_out=e, n_out=e)
+        a.update(kw)
+        with pytest.raises(M.ExpertError) as err:
+            M.block_norm_dev(a.pop("planes"), a.pop("residual"), a.pop("rows"), a.pop("width"), **a)
+        assert err.value.code == 1
