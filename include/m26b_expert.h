@@ -377,10 +377,10 @@ uint64_t m26b_linear_workspace_bytes(const m26b_linear* l, uint32_t rows);
 typedef struct m26b_linear_args {
     const void* x;              /* device [rows][k], rows x_pitch elements apart (0: dense) */
     const uint8_t* x_scales;    /* x_dtype 2: device [rows][k/32] UE8M0, dense; else unused */
-    void* y;                    /* device [rows][n], rows y_pitch elements apart (0: dense) */
+    void* y;                    /* device [rows][n], rows y_pitch elements apart (0: dense); overlaps no other argument */
     void* workspace;            /* device, 128-byte aligned, at least m26b_linear_workspace_bytes(rows). One call at a time: calls that */
     uint64_t workspace_bytes;   /* may overlap, or captured graphs that may run together, each need their own. No use between calls. */
-    uint32_t* fault_dev;        /* receives code 3 (ORed) if a bounded wait inside the kernel ran out; y is undefined then */
+    uint32_t* fault_dev;        /* device, 4-byte aligned: receives code 3 (ORed) if a bounded wait inside the kernel ran out; y is undefined then */
     uint64_t x_pitch, y_pitch;
     uint32_t rows;
     int32_t x_dtype;            /* 0 BF16, 2 E4M3 */

@@ -346,8 +346,9 @@ int m26b_linear_dev(const m26b_linear* l, const m26b_linear_args* args, void* st
         set_msg(err, errlen, "m26b linear: bad pointers/pitch/rows");
         return 1;
     }
-    if ((bf16 && reinterpret_cast<uintptr_t>(in.x) % 2) || reinterpret_cast<uintptr_t>(in.y) % (in.y_dtype ? 4 : 2)) {
-        set_msg(err, errlen, "m26b linear: x or y is not aligned to its element size");
+    if ((bf16 && reinterpret_cast<uintptr_t>(in.x) % 2) || reinterpret_cast<uintptr_t>(in.y) % (in.y_dtype ? 4 : 2) ||
+        reinterpret_cast<uintptr_t>(in.fault_dev) % 4) {
+        set_msg(err, errlen, "m26b linear: x, y or the fault word is not aligned to its element size");
         return 1;
     }
     if (!in.workspace || reinterpret_cast<uintptr_t>(in.workspace) % 128 || in.workspace_bytes < m26b_linear_workspace_bytes(l, rows)) {

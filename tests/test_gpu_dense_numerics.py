@@ -205,3 +205,19 @@ def test_far_gates_of_other_rows_change_nothing(torch):
     got = run(x2, rows)
     torch.cuda.synchronize()
     assert torch.equal(got[0::2], want[0::2])
+
+
+def test_an_unaligned_fault_word_is_refused(torch):
+    import mimo26f_afd_b200 as M
+
+    n, k = 64, 64
+    layer = M.Linear.new(*D.make_weights(torch, n, k, D.gen(torch, 1)), n, k)
+    x, y = torch.zeros(4, k, dtype=torch.bfloat16, device="cuda"), torch.zeros(4, n, device="cuda")
+    ws, f = torch.empty(layer.workspace_bytes(4), dtype=torch.uint8, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    for off in (1, 2, 3):
+        with pytest.raises(M.ExpertError) as e:
+            M.linear_dev(layer, x, 4, y, y_dtype=1, workspace=ws, fault=f.data_ptr() + off)
+        assert e.value.code == 1
+    M.linear_dev(layer, x, 4, y, y_dtype=1, workspace=ws, fault=f.data_ptr() + 4)
+    torch.cuda.synchronize()
+    assert f.tolist() == [0, 0]
