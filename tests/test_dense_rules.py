@@ -142,3 +142,26 @@ def test_no_rows_of_empty_tensors_are_no_work():
         with pytest.raises(M.ExpertError) as err:
             M.block_norm_dev(a.pop("planes"), a.pop("residual"), a.pop("rows"), a.pop("width"), **a)
         assert err.value.code == 1
+
+
+# Requests that CTA pairs run, and the token tile they run with: (BF16, gated, n, k, tokens, tile). Tiles of up to 128 tokens have one scale block
+# per piece, wider ones two.
+PAIR_SHAPES = [
+    (True, False, 305, 4320, 2354, 64), (True, False, 268, 6688, 3645, 112), (True, False, 13250, 1312, 451, 128), (True, False, 9928, 1056, 143, 144),
+    (True, False, 10709, 4064, 182, 192), (True, False, 1549, 32, 4038, 224), (True, True, 129, 4544, 2324, 64), (True, True, 14964, 416, 238, 128),
+    (True, True, 4867, 1088, 141, 144), (True, True, 5621, 4192, 178, 192), (True, True, 14241, 32, 132, 224),
+    (False, False, 260, 6720, 2364, 64), (False, False, 3659, 3008, 1070, 128), (False, False, 564, 2528, 3139, 144), (False, False, 9579, 3808, 145, 160),
+    (False, False, 14409, 128, 395, 256), (False, True, 139, 5440, 2346, 64), (False, True, 519, 3104, 3615, 128), (False, True, 4847, 2496, 134, 144),
+    (False, True, 14549, 32, 137, 256),
+]
+
+
+def image_tiles(n, gated):
+    """128-row tiles of a weight image: an even number; 64 features each when gated, 128 otherwise."""
+    return -(-n // (128 if gated else 256)) * 2
+
+
+def test_the_pair_shapes_run_on_pairs(rules):
+    for bf16, gated, n, k, rows, tile in PAIR_SHAPES:
+        assert rules.pair_tile(image_tiles(n, gated), -(-k // 128), rules.b200, 148, int(bf16), rows) == tile
+    assert {t <= 128 for *_, t in PAIR_SHAPES} == {True, False} and {t for *_, t in PAIR_SHAPES} >= {64, 224, 256}
