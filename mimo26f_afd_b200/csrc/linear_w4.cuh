@@ -322,8 +322,11 @@ struct LinearTile {
     static constexpr int kRedBytes = B_ROWS * kTileM * 4;                  // partial sums of a split K
     static constexpr int kFit = ((kCtasPerSm == 2 ? 111 : 224) * 1024 - kRedBytes) / kStageBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
-    static constexpr uint32_t kCols = kN + 32 <= 64 ? 64 : kN + 32 <= 128 ? 128 : kN + 32 <= 256 ? 256 : 512;   // two scale slots of 16 columns
-    static_assert(kStages >= 3, "too few stages");
+    // tensor memory: the accumulators and, above them, a scale slot per stage - 4 columns of weights, 4 per block of tokens. A stage is filled again
+    // only after the MMAs that read it, so its slot's next copies find those MMAs done.
+    static constexpr uint32_t kSfStride = 4 + 4 * kSfb, kNeed = kN + kStages * kSfStride;
+    static constexpr uint32_t kCols = kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : kNeed <= 256 ? 256 : 512;
+    static_assert(kStages >= 3 && kNeed <= 512 && kCtasPerSm * kCols <= 512, "too few stages, or more tensor memory than an SM has");
 };
 template <int B_ROWS, int PIECES>
 struct LinearSmem {
@@ -531,7 +534,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             for (uint32_t c = c0; c < c1; ++c) {
                 if (!mbar_wait(&s.full[stage], phase, abort_flag)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t t_sf = tb + T::kN + (c & 1u) * 16u;       // consecutive chunks alternate between two scale slots
+                const uint32_t t_sf = tb + T::kN + stage * T::kSfStride;
                 tc_cp_scales(t_sf, sfa_desc0 + stage * (sizeof(s.sfa[0]) >> 4));
 #pragma unroll
                 for (int b = 0; b < T::kSfb; ++b) tc_cp_scales(t_sf + 4 + 4 * b, sfb_desc0 + stage * (sizeof(s.sfb[0]) >> 4) + b * (kScaleBlockBytes >> 4));
@@ -627,12 +630,13 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 // item's MMAs run meanwhile. Barriers as in gemm_mx_pair.cuh: loads of both CTAs report to the first CTA's `full`.
 constexpr uint32_t kLpMaxTokens = 256;
 constexpr int kLpEpiWarps = 16, kLpThreads = 64 + 32 * kLpEpiWarps;
-constexpr uint32_t kLpSfStride = 32;                       // a scale slot: 4 columns of weights, 8 per piece of tokens
 template <int PIECES>
 struct LinearPairTile {
     static constexpr uint32_t kTokens = PIECES == 2 ? 224 : kLpMaxTokens;       // widest token tile; a piece's accumulator columns
-    static constexpr uint32_t kSf = PIECES * kTokens, kSfSlots = (kTmemCols - kSf) / kLpSfStride;    // scale slots above the accumulators
-    static_assert(kSfSlots >= 2 && 4 + 8 * PIECES <= kLpSfStride, "consecutive chunks use different slots");
+    // scale slots above the accumulators: 4 columns of weights, 8 per piece of tokens, one per stage or as many as there is room for
+    static constexpr uint32_t kStages = PIECES == 2 ? 4 : 6, kSf = PIECES * kTokens, kSfStride = 4 + 8 * PIECES;
+    static constexpr uint32_t kSfRoom = (kTmemCols - kSf) / kSfStride, kSfSlots = kSfRoom < kStages ? kSfRoom : kStages;
+    static_assert(kSfSlots >= 3, "two chunks' MMAs at work while a third's scales are copied");
 };
 
 struct LinearPairMaps {
@@ -643,7 +647,7 @@ struct LinearPairMaps {
 };
 template <int PIECES>
 struct LinearPairSmem {
-    static constexpr int kStages = PIECES == 2 ? 4 : 6;
+    static constexpr uint32_t kStages = LinearPairTile<PIECES>::kStages;
     static constexpr uint32_t kPieceBytes = LinearPairTile<PIECES>::kTokens / 2 * 128;
     alignas(1024) uint8_t a[kStages][kTileM * 128];
     alignas(1024) uint8_t b[kStages][PIECES * kPieceBytes];
@@ -745,6 +749,7 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
         grid_dep_wait();             // bounded waits start when the stream's earlier kernels have ended, however long they take
         if (rank == 0 && elect_one()) {
             uint32_t stage = 0, phase = 0, local = 0, slot = 0;
+            uint32_t issued = 0, old_stage = 0, old_phase = 0;       // chunks issued; the one whose scale slot comes next
             bool ok = true;
             const uint64_t a_desc0 = desc_sw128(smem_u32(s.a[0])), b_desc0 = desc_sw128(smem_u32(s.b[0]));
             const uint64_t sfa_desc0 = desc_scale_block(smem_u32(s.sfa[0])), sfb_desc0 = desc_scale_block(smem_u32(s.sfb[0]));
@@ -755,9 +760,17 @@ linear_pair_kernel(const __grid_constant__ LinearPairMaps maps, const LinearArgs
                 tc_fence_after();
                 for (uint32_t c = 0; c < p.chunks; ++c) {
                     if (!mbar_wait(&s.full[stage], phase, abort_flag)) { ok = false; break; }
+                    if constexpr (T::kSfSlots < kStages) {
+                        // with fewer slots than stages a refilled stage does not yet say that the slot's last MMAs are done: their commit does
+                        if (issued >= T::kSfSlots) {
+                            if (!mbar_wait(&s.empty[old_stage], old_phase, abort_flag)) { ok = false; break; }
+                            if (++old_stage == kStages) { old_stage = 0; old_phase ^= 1u; }
+                        }
+                        ++issued;
+                    }
                     tc_fence_after();
-                    const uint32_t t_sf = tb + T::kSf + slot * kLpSfStride;
-                    slot = (slot + 1) % T::kSfSlots;
+                    const uint32_t t_sf = tb + T::kSf + slot * T::kSfStride;
+                    if (++slot == T::kSfSlots) slot = 0;
                     tc_cp_scales_pair(t_sf, sfa_desc0 + stage * (sizeof(s.sfa[0]) >> 4));
                     const uint64_t sfb_d = sfb_desc0 + stage * (sizeof(s.sfb[0]) >> 4);
 #pragma unroll
