@@ -32,7 +32,8 @@ template <int B_ROWS>
 cudaError_t linear_room(int sms, uint32_t (&room)[4]) {
     using T = LinearTile<B_ROWS, 2>;
     const int smem = int(sizeof(LinearSmem<B_ROWS, 2>)) + 1024;
-    const cudaError_t e = cudaFuncSetAttribute(linear_room_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // the most a CTA may have, whatever is asked: another thread may be between its setting and its asking
+    const cudaError_t e = cudaFuncSetAttribute(linear_room_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
     if (e != cudaSuccess) return e;
     room[0] = uint32_t(sms * T::kCtasPerSm);
     for (uint32_t log_size = 1; log_size < 4; ++log_size) {

@@ -221,3 +221,30 @@ def test_an_unaligned_fault_word_is_refused(torch):
     M.linear_dev(layer, x, 4, y, y_dtype=1, workspace=ws, fault=f.data_ptr() + 4)
     torch.cuda.synchronize()
     assert f.tolist() == [0, 0]
+
+
+def test_handles_made_by_several_threads_run_the_same_kernels(torch):
+    """What a handle knows of the device does not depend on who else asks: the same K split, so the same bits."""
+    import threading
+
+    import mimo26f_afd_b200 as M
+
+    n, k, rows = 256, 4096, 9
+    g = D.gen(torch, 30)
+    w, s = D.make_weights(torch, n, k, g)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(torch.bfloat16)
+    want = D.Runner(torch, M.Linear.new(w, s, n, k), rows)(x, rows)
+    torch.cuda.synchronize()
+    layers = [[] for _ in range(8)]
+
+    def make(to):
+        for _ in range(20):
+            to.append(M.Linear.new(w, s, n, k))
+
+    threads = [threading.Thread(target=make, args=(to,)) for to in layers]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for layer in sum(layers, []):
+        assert torch.equal(D.Runner(torch, layer, rows)(x, rows), want)
