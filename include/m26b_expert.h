@@ -357,14 +357,14 @@ int m26b_plan_static(const int32_t* ids, const float* weights, uint32_t rows, in
  *   workspace_bytes: device bytes m26b_linear_dev needs for `rows` tokens (0 for 0 rows); grows with rows up to 8,192.
  *   linear_dev: x [rows][k], BF16 or E4M3 with UE8M0 scales per 32 k -> y [rows][n], BF16 (one rounding, nearest even) or
  *              FP32. Only y's n columns of `rows` rows are written. One token to a prefill batch (passes of 8,192; at most
- *              2^31 - 1 rows); 0 rows is no work. BF16 activations are not quantised: a K32 block enters the product as two E4M3
- *              pieces that equal it exactly, save for elements below 2^-13 of the block's largest, which carry an error of
- *              at most 2^-21 of that largest. Products accumulate in FP32; a sum beyond FP32 is infinite, or NaN. The activation is within
- *              2^-19 of itself (relative) whatever its argument. A row with an infinity, a NaN (or, for E4M3, a NaN
- *              code or scale byte 255) in it is NaN in all its outputs. A row's result does not change with the other rows'
- *              values. Nothing is allocated, nothing is synchronised, and a call can be captured into a graph; the handle
- *              must stay alive until the work is done, the argument record is read before the call returns. Enqueued on
- *              `stream` (NULL = the default stream). */
+ *              2^31 - 1 rows); 0 rows is no work. A K32 block of BF16 activations enters the product as two E4M3 pieces. They equal it
+ *              exactly, save for elements below 2^-13 of the block's largest: those carry an error of at most 2^-21 of that
+ *              largest, so beside an element four orders above them they keep fewer bits than BF16 has. Products accumulate in FP32;
+ *              a sum beyond FP32 is infinite, or NaN. The activation is within 2^-19 of itself whatever its argument. A row with an
+ *              infinity, a NaN (or, for E4M3, a NaN code or scale byte 255) in it is NaN in all its outputs. A row's result does
+ *              not change with the other rows' values. Nothing is allocated, nothing is synchronised, and a call can be captured
+ *              into a graph; the handle must stay alive until the work is done, the argument record is read before the call
+ *              returns. Enqueued on `stream` (NULL = the default stream). */
 typedef struct m26b_linear m26b_linear;
 int m26b_linear_new(const uint8_t* w, const uint8_t* s, uint32_t n, uint32_t k, m26b_linear** out, char* err, size_t errlen);
 int m26b_linear_new_gated(const uint8_t* gate_w, const uint8_t* gate_s, const uint8_t* up_w, const uint8_t* up_s, uint32_t n, uint32_t k,
@@ -397,7 +397,7 @@ int m26b_linear_dev(const m26b_linear* l, const m26b_linear_args* args, void* st
  * dtypes: 0 = BF16, 1 = FP32; pitches are in elements, 0 means dense rows. FP32 throughout, one rounding per output; n is
  * computed from h before h is rounded. A sum of squares beyond FP32 is rescaled, so finite rows have finite norms. The
  * argument record is read before the call returns. Enqueued on `stream` (NULL = the default stream); outputs other than
- * h_out == residual must not overlap inputs. 0 rows is no work. */
+ * h_out == residual must not overlap inputs. 0 rows is no work (the arguments are checked all the same). */
 typedef struct m26b_block_norm_args {
     const void* planes[8];      /* device, the block's output: one plane per rank [rows][width], y_dtype, y_pitch */
     const void* post_w;         /* [width] of w_dtype, or NULL: no norm of u */

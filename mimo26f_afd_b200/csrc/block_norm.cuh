@@ -8,8 +8,8 @@
 // in registers between the two reductions. Everything is FP32 from the loads to the single rounding of each output.
 //
 // What bounds it: HBM traffic (planes + residual in, h and n out); about twelve operations per element. Measured (BF16 plane, post
-// and pre norm): 8,192 x 4,096 with an FP32 residual stream 75 us = 5.4 TB/s, BF16 stream and a gate per element 60 us = 5.6 TB/s,
-// 8,192 x 4,095 dense rows 101 us = 4.0 TB/s, one row 3.5 us. Issue slots matter next: the row's shared factors are folded into one,
+// and pre norm): 8,192 x 4,096 with an FP32 residual stream 75 us = 5.4 TB/s, BF16 stream and a gate per element 61 us = 5.5 TB/s,
+// 8,192 x 4,095 dense rows 95 us = 4.2 TB/s, one row 3.5 us. Issue slots matter next: the row's shared factors are folded into one,
 // the root is rsqrtf, and what differs from call to call is asked per vector or per four elements.
 // Layout: rows on vector boundaries stay in registers (block_norm_kernel: a row belongs to a warp or a CTA, a thread owns PER
 // vectors of VEC elements, a row's worth apart, so that every access of a warp is one contiguous run); other and wider rows wait for

@@ -36,7 +36,8 @@ inline uint64_t linear_workspace(uint32_t k_pad, uint32_t rows) {
 // log2 of the CTAs that share a weight tile's K (a cluster): doubled while the clusters still run at once and each CTA keeps at least
 // two chunks. A GPC holds whole clusters only, so that fewer of them run at once than SMs over cluster size (of the 148 SMs here 33 clusters of
 // four and fifteen of eight with one CTA per SM, 71 and 33 with two), and what is left would run as a second round (100 tokens, 2,048 x
-// 2,048, sixteen clusters of eight: 15.2 us, of four: 8.3; 16 tokens, 4,224 x 16,384: 11.5 and 16.6). Powers of two: the divisions that other sizes need cost 0.3 us, more than they gain.
+// 2,048, sixteen clusters of eight: 15.2 us, of four: 8.3; 16 tokens, 4,224 x 16,384: 11.5 and 16.6). Powers of two: the divisions that
+// other sizes need cost 0.3 us, more than they gain.
 inline uint32_t linear_log_split(const LinearShape& L, uint64_t ctas, uint32_t per_sm, uint32_t chunks) {
     uint32_t log_split = 0;
     while (log_split < 3 && (ctas << (log_split + 1)) <= L.room[per_sm - 1][log_split + 1] && chunks >= 4u << log_split) ++log_split;
@@ -53,12 +54,13 @@ inline bool linear_direct(const LinearShape& L, bool bf16, uint32_t rows) {
     return ctas <= L.sms && per_cta * (rows < 128 ? rows : 128) <= (bf16 ? 256u : 512u);
 }
 // Token tile of the CTA-pair kernel (`ctas`: how many of its CTAs run at once) for a request, or 0 if single CTAs (which can split K)
-// finish it sooner, by cycles: rounds of items over the GPU x cycles per item. A 128-wide chunk costs a pair 4 x pieces MMAs, each the slower of its math (tile / 2
-// cycles) and of shared memory at 128 B/clk (weight rows 32 cycles, token rows tile / 8, its share of filling the stage); a
-// single CTA of 128 tokens 768 (two pieces) or 512 cycles, shared memory again. The constants are what start, end and
-// hand-over of an item cost. A tile narrower than the widest has to win by a tenth: it is more work in all, and the GPU is at
-// its power limit. Measured (4,096 x 4,096, pairs / single CTAs): 512 tokens 22.1 / 20.3 us, 768 26.6 / 31.1, E4M3 512 17.9 / 15.0,
-// 1,024 21.5 / 28.9; 1,536 tokens with tiles of 176 / 256: 46.0 / 53.1 us.
+// finish it sooner, by cycles: rounds of items over the GPU x cycles per item. A 128-wide chunk costs a pair 4 x pieces MMAs, each the
+// slower of its math (tile / 2 cycles) and of shared memory at 128 B/clk (weight rows 32 cycles, token rows tile / 8, its share of
+// filling the stage); a single CTA of 128 tokens 768 (two pieces) or 512 cycles, shared memory again. The constants are what start, end
+// and hand-over of an item cost. A tile narrower than the widest has to win by a tenth: it is more work in all, and the GPU is at
+// its power limit (2,048 E4M3 tokens with tiles of 240, 2 % fewer cycles by this count, take 35.5 us, of 256 34.3). Measured (4,096 x
+// 4,096, the best pairs / single CTAs): 512 tokens 22.7 / 20.2 us, 768 27.7 / 35.1, 1,024 39.2 / 40.9, 2,048 69.6 / 78.2; E4M3 512 15.8 /
+// 12.6, 1,024 19.0 / 25.3.
 inline uint32_t linear_pair_tile(const LinearShape& L, uint32_t ctas, bool bf16, uint32_t rows) {
     if (rows <= 128 || ctas < 2) return 0;
     const uint64_t pairs = ctas / 2, m_pairs = L.tiles / 2, pieces = bf16 ? 2 : 1;

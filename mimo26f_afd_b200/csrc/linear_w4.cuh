@@ -10,8 +10,8 @@
 // every element of at least 2^-6 * 2^s, so of at least 2^-13 of its block's largest; below, the pair is off by at most
 // 2^-14 * 2^s < 2^-21 of that largest element, what one FP32 rounding of a partial sum costs. The products of both pieces
 // accumulate in FP32 tensor memory: the weights are fetched once and the tensor pipe runs them twice, at the FP8 rate, which is
-// the rate of a BF16 product - with no dequantised copy of the weights anywhere. Quantised activations (E4M3 rows with
-// UE8M0 K32 scales) take one piece.
+// the rate of a BF16 product - with no dequantised copy of the weights anywhere. Each piece has accumulators of its own. Quantised
+// activations (E4M3 rows with UE8M0 K32 scales) take one piece.
 //
 // A K32 block with an infinity or a NaN becomes a block of NaN: every output of that row is NaN.
 //
@@ -621,7 +621,7 @@ linear_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 // cta_group::2: two CTAs of a cluster run one MMA of M = 256 (128 weight rows each) x N = `tile` tokens (at most 256 with one piece, 224
 // with two), half of the token rows in each CTA's shared memory. What bounds a block-scaled MMA at prefill is shared memory, which feeds the
 // operands (128 B/clk) and takes the loads: per 128-wide chunk and CTA, 224 tokens of two pieces read 60 KB and fill 44 KB in 896 cycles
-// of math, 119 B/clk; 128 tokens wide it would be 144, a single CTA of 128 x 128 tokens 192.
+// of math, 119 B/clk; 128 tokens wide it would be 160, a single CTA of 128 x 128 tokens 224.
 // Each piece has accumulator columns of its own, added once in the epilogue. The tensor core truncates its running sum to FP32 after every
 // MMA. The leading pieces' products lie on a coarse grid, so that little falls off; with the second pieces' sixteen times finer
 // products in the same column every step loses a part of a unit in the last place, towards zero (2,048 tokens, 4,096 x 4,096, FP32
